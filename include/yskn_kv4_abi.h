@@ -414,6 +414,72 @@ YSKN_KV4_API int yskn_kv8_attention_ws(const yskn_kv8_attn_args* a, int act_dtyp
 YSKN_KV4_API int yskn_kv8_combine(const float* d_pm, const float* d_pl, const float* d_pacc, int splits, int M, int nh, const void* d_gate,
                                   void* d_o16, int act_dtype, int inverse_rotate, void* cuda_stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * A paged cache of 16-bit rows, for many sequences whose lengths nobody knows ahead.  One layer's rows lie in pages:
+ *   k, v    f16 or bf16 [pages][kvh][page][hd]     keys rotated when they are appended
+ *   kmean   the same type [pages][kvh][hd], or NULL     mean key of every page whose last row has been appended
+ * page is 16, 32, 64 or 128 tokens, hd 128 or 256; pages * kvh * page < 2^31; the arrays are 16-byte aligned.  The caller fills the members up to
+ * `dtype` and calls yskn_kv4_paged_init once, which checks them and writes the tensor maps of the arrays into `maps`; the struct is then passed as it is. */
+typedef struct yskn_paged_cache {
+  void* k; void* v; void* kmean;
+  int pages, kvh, page, hd, dtype;             /* dtype: YSKN_KV4_F16 or YSKN_KV4_BF16 */
+  int ready;                                   /* set by yskn_kv4_paged_init */
+  uint64_t maps[4][16];
+} yskn_paged_cache;
+YSKN_KV4_API int yskn_kv4_paged_init(yskn_paged_cache* c);
+
+/* The rows of a pass (device arrays).  table [seqs][blocks]: the page that holds block b of sequence s; entries outside [0, pages) name none.
+ * Row r belongs to sequence seq[r] and stands at position pos[r].  A row whose seq is outside [0, seqs) is padding: nothing is read or written for it. */
+typedef struct yskn_paged_rows {
+  const int* table; int seqs, blocks;
+  const int* seq; const int* pos; int rows;
+} yskn_paged_rows;
+
+/* Rotates keys (and queries) at each row's position and writes keys and values into their pages.  k_in, v_in: rows [kvh][hd] at a distance of k_stride,
+ * v_stride elements; q_in: rows [nh][hd] at a distance of q_stride, rotated into q_out [rows][nh][hd] (q_in NULL: no queries).  Channels c and c + rd/2
+ * (c < rd/2) turn by entry [pos][c] of `rope`, (cos, sin) pairs fp32 [rope_rows][rd/2] as yskn_kv4_rope_table writes them, in fp32, rounded once;
+ * rd a multiple of 16, at most hd, 0: no rotation.  All rows have the cache's type; pointers and strides are multiples of 16 bytes.
+ * A row at a position that has no page (or, with rd > 0, no entry of the table: negative, or beyond rope_rows) is left out, its query too where the position
+ * has no entry.  With kmean the mean key (fp32 sum) of each page whose last row is among these rows is written by a second launch.
+ * Two rows of one call must not share a place. */
+typedef struct yskn_paged_append_args {
+  const void* k_in; const void* v_in; const void* q_in; void* q_out;
+  int64_t k_stride, v_stride, q_stride;
+  const float* rope; int rope_rows, rd, nh;
+} yskn_paged_append_args;
+YSKN_KV4_API int yskn_kv4_paged_append(const yskn_paged_cache* c, const yskn_paged_rows* r, const yskn_paged_append_args* a, void* cuda_stream);
+
+/* The blocks that a row attends to, chosen by a cheap score.  Of the blocks in front of the row's last one (block pos / page, which is always taken) the
+ * `take` - 1 with the highest score, ties to the lowest block: score = max over the heads h of the kv-head's group of q_h . kmean[page], summed in fp64 (a
+ * score that is not a number counts as the lowest; blocks without a page are no candidates).  ids [rows][kvh][take]: the chosen blocks in rising order, then -1;
+ * for a padding row nothing is written, for a row at a negative position all -1.  A position beyond the table counts as the table's last.  q: rows [nh][hd] of the
+ * cache's type at a distance of q_stride elements, 16-byte aligned.  2 <= take <= 1024; nh / kvh <= 16. */
+typedef struct yskn_paged_select_args {
+  const void* q; int64_t q_stride; int nh, take;
+  int* ids; void* workspace; size_t workspace_bytes;
+} yskn_paged_select_args;
+YSKN_KV4_API int yskn_kv4_paged_select(const yskn_paged_cache* c, const yskn_paged_rows* r, const yskn_paged_select_args* a, void* cuda_stream);
+
+/* Attention of every row over the tokens 0 .. pos of its sequence: o16 [rows][nh][hd] = softmax(qscale * q . k) v, statistics and sums in fp32, weights rounded
+ * to the cache's type for the products.  q: rows [nh][hd] (rotated) at a distance of q_stride elements.  nh / kvh <= 16.  A position beyond the table counts as the
+ * table's last; tokens without a page are not seen; a row that sees nothing becomes zeros; a padding row is left as it is.  What pages hold beyond a
+ * sequence's tokens is never used, whatever it is.
+ *   shared > 0  (a multiple of page): the first `shared` tokens lie on the same pages in the table of every row that has that many (read through the first
+ *               such row's): they are read once for all rows, on the tcgen05 tensor cores, and joined with what each row has behind them.  A shorter row attends by itself.
+ *   ids         [rows][kvh][take], shared = 0: a row sees only the tokens of these blocks (in any order; entries outside the table, or beyond the row's last
+ *               block, name none; a block named twice counts twice).
+ * The sum of a row is split where the work of all rows is shared out evenly, so its last bit depends on the other rows of the call.
+ * workspace: yskn_kv4_paged_workspace_bytes, 256-byte aligned, for one call at a time; its contents need not survive the call's work on the stream. */
+typedef struct yskn_paged_attn_args {
+  const void* q; int64_t q_stride; int nh; float qscale; void* o16;
+  int shared; const int* ids; int take;
+  void* workspace; size_t workspace_bytes;
+} yskn_paged_attn_args;
+YSKN_KV4_API int yskn_kv4_paged_attention(const yskn_paged_cache* c, const yskn_paged_rows* r, const yskn_paged_attn_args* a, void* cuda_stream);
+/* Bytes that yskn_kv4_paged_attention over `rows` rows needs with this `shared`, and, where blocks > 0, yskn_kv4_paged_select over a table of so many blocks (the larger
+ * of the two); 0 for a shape that is refused. */
+YSKN_KV4_API size_t yskn_kv4_paged_workspace_bytes(const yskn_paged_cache* c, int rows, int nh, int shared, int blocks);
+
 #ifdef __cplusplus
 }
 #endif

@@ -71,6 +71,30 @@ class PeerExchangeC(C.Structure):     # yskn_kv4_peer_exchange
     _fields_ = [("buf", C.c_void_p * 8), ("world", C.c_int), ("rank", C.c_int)]
 
 
+class PagedCacheC(C.Structure):       # yskn_paged_cache
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("kmean", C.c_void_p), ("pages", C.c_int), ("kvh", C.c_int), ("page", C.c_int), ("hd", C.c_int),
+                ("dtype", C.c_int), ("ready", C.c_int), ("maps", (C.c_uint64 * 16) * 4)]
+
+
+class PagedRowsC(C.Structure):        # yskn_paged_rows
+    _fields_ = [("table", C.c_void_p), ("seqs", C.c_int), ("blocks", C.c_int), ("seq", C.c_void_p), ("pos", C.c_void_p), ("rows", C.c_int)]
+
+
+class PagedAppendArgsC(C.Structure):  # yskn_paged_append_args
+    _fields_ = [("k_in", C.c_void_p), ("v_in", C.c_void_p), ("q_in", C.c_void_p), ("q_out", C.c_void_p), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("q_stride", C.c_int64), ("rope", C.c_void_p), ("rope_rows", C.c_int), ("rd", C.c_int), ("nh", C.c_int)]
+
+
+class PagedSelectArgsC(C.Structure):  # yskn_paged_select_args
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64), ("nh", C.c_int), ("take", C.c_int), ("ids", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
+class PagedAttnArgsC(C.Structure):    # yskn_paged_attn_args
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64), ("nh", C.c_int), ("qscale", C.c_float), ("o16", C.c_void_p), ("shared", C.c_int),
+                ("ids", C.c_void_p), ("take", C.c_int), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 # name -> (restype, argtypes); every symbol include/yskn_kv4_abi.h declares
 PROTOTYPES = {
     "yskn_kv4_last_error": (C.c_char_p, []),
@@ -127,6 +151,11 @@ PROTOTYPES = {
     "yskn_kv8_workspace_bytes": (C.c_size_t, [C.POINTER(Kv8AttnArgsC)]),
     "yskn_kv8_attention_ws": (C.c_int, [C.POINTER(Kv8AttnArgsC), C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
     "yskn_kv8_combine": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
+    "yskn_kv4_paged_init": (C.c_int, [C.POINTER(PagedCacheC)]),
+    "yskn_kv4_paged_append": (C.c_int, [C.POINTER(PagedCacheC), C.POINTER(PagedRowsC), C.POINTER(PagedAppendArgsC), C.c_void_p]),
+    "yskn_kv4_paged_select": (C.c_int, [C.POINTER(PagedCacheC), C.POINTER(PagedRowsC), C.POINTER(PagedSelectArgsC), C.c_void_p]),
+    "yskn_kv4_paged_attention": (C.c_int, [C.POINTER(PagedCacheC), C.POINTER(PagedRowsC), C.POINTER(PagedAttnArgsC), C.c_void_p]),
+    "yskn_kv4_paged_workspace_bytes": (C.c_size_t, [C.POINTER(PagedCacheC), C.c_int, C.c_int, C.c_int, C.c_int]),
     "yskn_kv4_attention_host": (C.c_int, [C.c_void_p, C.POINTER(KvLayerC), C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p,
                                           C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, C.c_int, C.c_void_p, C.c_int,
                                           C.c_void_p]),

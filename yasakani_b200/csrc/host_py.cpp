@@ -10,7 +10,9 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <climits>
 #include <cstdlib>
 #include "../../include/yskn_kv4_abi.h"
 
@@ -302,13 +304,114 @@ FN(tb_attention) {  // profile, q16, k_pay, k_side, v_pay, v_side, grp_k, grp_v,
   });
 }
 
+// ---- the paged 16-bit cache (paged.py): v[0] the ctypes struct, v[1] the tensor of keys (device and type of the call)
+struct Paged { yskn_paged_cache c; yskn_paged_rows r; at::ScalarType type; c10::Device dev; };
+const at::Tensor& paged_tensor(const Paged& P, PyObject* o, at::ScalarType t, const char* what) {
+  const at::Tensor& x = tensor(o, what);
+  if (x.scalar_type() != t) { PyErr_Format(PyExc_TypeError, "%s: wrong type", what); throw PyFail{}; }
+  if (x.device() != P.dev) { PyErr_Format(PyExc_AssertionError, "%s: not on the cache's device", what); throw PyFail{}; }
+  return x;
+}
+Paged paged_of(PyObject* cache, PyObject* keys, PyObject* table, PyObject* seq, PyObject* pos) {
+  const at::Tensor& k = tensor(keys, "cache");
+  Paged P{{}, {}, k.scalar_type(), k.device()};
+  Py_buffer b;
+  if (PyObject_GetBuffer(cache, &b, PyBUF_SIMPLE)) throw PyFail{};
+  const bool ok = b.len == (Py_ssize_t)sizeof(P.c);
+  if (ok) memcpy(&P.c, b.buf, sizeof(P.c));
+  PyBuffer_Release(&b);
+  if (!ok) fail(PyExc_TypeError, "cache: a PagedCache is needed");
+  const at::Tensor &t = paged_tensor(P, table, at::kInt, "table"), &s = paged_tensor(P, seq, at::kInt, "seq"), &p = paged_tensor(P, pos, at::kInt, "pos");
+  if (t.dim() != 2 || s.dim() != 1 || p.dim() != 1 || s.size(0) != p.size(0)) fail(PyExc_ValueError, "table [sequences][blocks], seq and pos [rows]");
+  check_dev(t, "table"); check_dev(s, "seq"); check_dev(p, "pos");
+  if (t.size(0) > INT_MAX || t.size(1) > INT_MAX || s.size(0) > INT_MAX) fail(PyExc_OverflowError, "an argument does not fit a C int");
+  P.r = yskn_paged_rows{(const int*)t.data_ptr(), (int)t.size(0), (int)t.size(1), (const int*)s.data_ptr(), (const int*)p.data_ptr(), (int)s.size(0)};
+  return P;
+}
+struct HeadRows { void* p; int64_t stride; int heads; };
+HeadRows head_rows(const Paged& P, PyObject* o, int heads, const char* what) {     // [rows][heads][hd], heads and channels contiguous; heads < 0: any number
+  const at::Tensor& t = paged_tensor(P, o, P.type, what);
+  if (t.dim() != 3 || t.size(0) != P.r.rows || t.size(2) != P.c.hd || (heads >= 0 && t.size(1) != heads) || t.size(1) > INT_MAX) {
+    PyErr_Format(PyExc_ValueError, "%s: [rows][heads][hd] for the cache's heads and the rows of seq", what); throw PyFail{};
+  }
+  if (t.stride(2) != 1 || (t.size(1) > 1 && t.stride(1) != P.c.hd)) { PyErr_Format(PyExc_AssertionError, "%s: the heads of a row must be contiguous", what); throw PyFail{}; }
+  const int64_t least = t.size(1) * P.c.hd;
+  return HeadRows{t.data_ptr(), t.size(0) > 1 ? t.stride(0) : least, (int)t.size(1)};
+}
+// The call runs with the cache's device current, on that device's current stream where none is given.
+template <class F> PyObject* paged_call(const Paged& P, PyObject* stream, const char* who, F f) {
+  const c10::cuda::CUDAGuard guard(P.dev);
+  const cudaStream_t st = stream_of(stream);
+  return call(who, [&] { return f(st); });
+}
+struct Buf { void* p; size_t bytes; };
+Buf paged_ws(const Paged& P, PyObject* o) {
+  const at::Tensor& t = tensor(o, "ws");
+  if (t.device() != P.dev) fail(PyExc_AssertionError, "ws: not on the cache's device");
+  check_dev(t, "ws");
+  return Buf{t.data_ptr(), (size_t)t.nbytes()};
+}
+
+FN(paged_append) {                                       // cache, keys, table, k, v, seq, pos, rope, rd, q, q_out, stream
+  return guarded(n, 12, [&]() -> PyObject* {
+    const Paged P = paged_of(v[0], v[1], v[2], v[5], v[6]);
+    const HeadRows k = head_rows(P, v[3], P.c.kvh, "k"), x = head_rows(P, v[4], P.c.kvh, "v");
+    yskn_paged_append_args a{k.p, x.p, nullptr, nullptr, k.stride, x.stride, 0, nullptr, 0, int_of(v[8]), 0};
+    if (v[7] != Py_None) {
+      const at::Tensor& rope = paged_tensor(P, v[7], at::kFloat, "rope");
+      check_dev(rope, "rope");
+      if (a.rd > 0) {                                    // [positions][rd / 2][2], or flat
+        if (rope.numel() % a.rd || rope.numel() / a.rd > INT_MAX) fail(PyExc_ValueError, "rope: fp32 [positions][rd / 2][2]");
+        a.rope = (const float*)rope.data_ptr(); a.rope_rows = (int)(rope.numel() / a.rd);
+      }
+    }
+    if (v[9] != Py_None) {
+      const HeadRows q = head_rows(P, v[9], -1, "q"), out = head_rows(P, v[10], q.heads, "q_out");
+      check_dev(tensor(v[10], "q_out"), "q_out");
+      a.q_in = q.p; a.q_out = out.p; a.q_stride = q.stride; a.nh = q.heads;
+    }
+    return paged_call(P, v[11], "yskn_kv4_paged_append", [&](cudaStream_t st) { return yskn_kv4_paged_append(&P.c, &P.r, &a, st); });
+  });
+}
+
+FN(paged_select) {                                       // cache, keys, table, seq, pos, q, ids, ws, stream
+  return guarded(n, 9, [&]() -> PyObject* {
+    const Paged P = paged_of(v[0], v[1], v[2], v[3], v[4]);
+    const HeadRows q = head_rows(P, v[5], -1, "q");
+    const at::Tensor& ids = paged_tensor(P, v[6], at::kInt, "ids");
+    check_dev(ids, "ids");
+    if (!is_shape(ids, P.r.rows, P.c.kvh, ids.dim() == 3 ? ids.size(2) : 0)) fail(PyExc_ValueError, "ids [rows][hkv][take]");
+    const Buf ws = paged_ws(P, v[7]);
+    const yskn_paged_select_args a{q.p, q.stride, q.heads, (int)std::min<int64_t>(ids.size(2), INT_MAX), (int*)ids.data_ptr(), ws.p, ws.bytes};
+    return paged_call(P, v[8], "yskn_kv4_paged_select", [&](cudaStream_t st) { return yskn_kv4_paged_select(&P.c, &P.r, &a, st); });
+  });
+}
+
+FN(paged_attention) {                                    // cache, keys, table, seq, pos, q, qscale, o16, shared, blocks, ws, stream
+  return guarded(n, 12, [&]() -> PyObject* {
+    const Paged P = paged_of(v[0], v[1], v[2], v[3], v[4]);
+    const HeadRows q = head_rows(P, v[5], -1, "q"), o = head_rows(P, v[7], q.heads, "o16");
+    check_dev(tensor(v[7], "o16"), "o16");
+    const Buf ws = paged_ws(P, v[10]);
+    yskn_paged_attn_args a{q.p, q.stride, q.heads, float_of(v[6]), o.p, int_of(v[8]), nullptr, 0, ws.p, ws.bytes};
+    if (v[9] != Py_None) {
+      const at::Tensor& ids = paged_tensor(P, v[9], at::kInt, "blocks");
+      check_dev(ids, "blocks");
+      if (!is_shape(ids, P.r.rows, P.c.kvh, ids.dim() == 3 ? ids.size(2) : 0)) fail(PyExc_ValueError, "blocks [rows][hkv][take]");
+      if (ids.size(2) < 1) fail(PyExc_ValueError, "blocks: no block at all");
+      a.ids = (const int*)ids.data_ptr(); a.take = (int)std::min<int64_t>(ids.size(2), INT_MAX);
+    }
+    return paged_call(P, v[11], "yskn_kv4_paged_attention", [&](cudaStream_t st) { return yskn_kv4_paged_attention(&P.c, &P.r, &a, st); });
+  });
+}
+
 PyObject* library(PyObject*, PyObject* const*, Py_ssize_t) {  // where the library this module calls is loaded
   return PyLong_FromVoidPtr((void*)yskn_kv4_last_error);
 }
 
 #define M_(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {M_(kv_append), M_(attention), M_(decode), M_(combine), M_(attention_ms), M_(attention_tc), M_(prefill_tc), M_(attn_post),
-                         M_(kv8_attention), M_(kv8_attention_tc), M_(kv8_combine), M_(tb_attention), M_(library), {nullptr, nullptr, 0, nullptr}};
+                         M_(kv8_attention), M_(kv8_attention_tc), M_(kv8_combine), M_(tb_attention), M_(paged_append), M_(paged_select), M_(paged_attention), M_(library), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host", "argument marshalling of the hot launchers", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -106,7 +106,10 @@ int yskn_kv4_device_status(int* status) {
   if (int rc = tc_status_fetch(&b)) return rc;
   int c = 0;
   if (int rc = merge_status_fetch(&c)) return rc;
-  *status = a ? a : (b ? b : c); return 0;
+  int d = 0, e = 0;
+  if (int rc = paged::attn_status_fetch(&d)) return rc;
+  if (int rc = paged::prefix_status_fetch(&e)) return rc;
+  *status = a ? a : b ? b : c ? c : d ? d : e; return 0;
 }
 
 int yskn_kv4_set_peer_wait_polls(unsigned polls) { set_peer_wait_polls(polls); return 0; }

@@ -133,6 +133,9 @@ int launch_kv8_attention_tc_ws(const yskn_kv8_attn_args& a, int act_dtype, void*
 int launch_kv8_combine(const float* pm, const float* pl, const float* pacc, int splits, int M, int nh, const void* gate, void* o16,
                        int act_dtype, int inverse_rotate, cudaStream_t st);
 
+// Paged 16-bit cache: status words of its attention kernels (paged_common.cuh has the rest)
+namespace paged { int attn_status_fetch(int* out); int prefix_status_fetch(int* out); }
+
 // Which attention kernel yskn_kv4_attention picks; set through yskn_kv4_set_algo (tests compare paths).
 enum Algo { ALGO_AUTO = 0, ALGO_SCALAR = 1, ALGO_MMA = 2 };
 int current_algo();

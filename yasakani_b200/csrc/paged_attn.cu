@@ -1,0 +1,546 @@
+// Attention of single rows over a paged 16-bit cache (sm_100a): batched decode, attention over chosen blocks, the rows' own part behind a shared prefix.
+//
+// Mathematics: o = sum_j p_j v_j / sum_j p_j, p_j = 2^(s q.k_j log2 e - m), m the running maximum; a tile of 64 tokens at a time, one pass over K and V.
+//
+// Bound: HBM.  A token of a kv-head costs 4 HD bytes and 2 G HD multiply-adds for the G <= 16 heads that share it, which is what warp-level tensor-core
+// tiles are for: S^T[16 tokens x 8 heads] = K Q^T, O^T[16 channels x 8 heads] += V^T P^T, keys and values straight from the swizzled tiles (ldmatrix).
+//
+// Work split.  The tiles of all (row, kv-head) pairs form one line, row after row, which the CTAs of a grid that fills the GPU share out evenly, whatever the lengths
+// are: no CTA has more than one tile above another.  A CTA's run covers parts of one or several pairs.  A pair that lies in one CTA is finished there; of a
+// pair that lies on several each CTA writes (m, l, O) to the piece number (CTA + pair), which is unique because along the line either number only grows, and
+// the merge kernel adds the pieces up.  Every CTA derives the line from the positions itself (a scan over at most ROWS rows).
+//
+// A CTA: one producer warp, four compute warps.  The producer asks for the tiles' pages by TMA (a box of min(page, 64) rows, 128-byte swizzle) into a ring of six
+// half stages, K and V in turn, ahead of the compute warps and across the borders of pairs; page numbers come 32 at a time.  The compute warps take 16 tokens
+// each for S, share the tile's maxima and weights through shared memory (two named barriers a tile), and take HD / 4 channels each for O, so no warp holds a copy of O.
+// hd 256: one CTA an SM (192 KB in flight); hd 128: two.
+//
+// Tokens that a row does not see: absent blocks are read outside the tensor map (zeros); what a page holds behind the sequence's end is zeroed in
+// shared memory before the product (a weight of 0 times an infinity would be none); scores are masked by selection.
+// Every wait is bounded; one that runs out sets the status word (7) and all warps walk to the end without waiting again.
+#include "paged_common.cuh"
+#include <algorithm>
+#include <cstring>
+
+namespace kv4 {
+namespace paged {
+
+__device__ int g_attn_status = 0;            // 0 ok; 7 = a bounded wait ran out
+
+namespace {
+
+constexpr int ROWS = 512;                    // rows of one launch
+constexpr int NSLOT = 6;                     // half stages of the ring: K, V, K, V, K, V
+constexpr int CW = 4, NT_ = (CW + 1) * 32;   // compute warps; threads
+
+struct AttnP {
+  Rows R; int rows, g, nh;
+  const uint16_t* q; long long qs; float cs; // cs = qscale * log2(e)
+  uint16_t* o16;
+  int shared; const int* ids; int take;
+  int* first; float* pm; float* pl; float* pacc;       // pieces
+  const float* qm; const float* ql; const float* qacc; int splits;     // partials over the shared prefix
+};
+
+template <int HD, int NT> struct Lay {
+  static constexpr int HALF = TILE * HD * 2, QP = HD * 2 + 16, PP = TILE * 2 + 16;   // bytes: a half stage; a row of Q; a row of P (paddings: eight rows on different banks)
+  static constexpr int OFF_Q = NSLOT * HALF, OFF_P = OFF_Q + 2 * NT * 8 * QP, OFF_MAX = OFF_P + 2 * NT * 8 * PP, OFF_L = OFF_MAX + 2 * CW * NT * 8 * 4;
+  static constexpr int OFF_BASE = OFF_L + CW * NT * 8 * 4, OFF_BAR = OFF_BASE + 3 * 4 * 4, OFF_SUM = OFF_BAR + 16 * 8 + 8, OFF_FIRST = OFF_SUM + 32;
+  static constexpr int TOTAL = OFF_FIRST + (ROWS + 1) * 4;
+  static constexpr int CTAS = HD == 256 ? 1 : 2;
+  static_assert(HALF % 1024 == 0 && OFF_BASE % 16 == 0 && OFF_BAR % 8 == 0 && CTAS * (TOTAL + 1024) <= 228 * 1024, "shared memory");
+};
+
+__device__ __forceinline__ void ldm4(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldm4t(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void stm2t(uint32_t a, uint32_t x, uint32_t y) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1,%2};" ::"r"(a), "r"(x), "r"(y) : "memory");
+}
+template <bool BF> __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (BF) asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+              : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+           : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// Tokens of a row that this kernel attends to by position: [start, vis); a row that has all of the shared prefix leaves that to the prefix kernel.
+__device__ __forceinline__ int start_of(const Place& w, int shared) { return shared > 0 && w.vis >= shared ? shared : 0; }
+__device__ __forceinline__ int tiles_of(const AttnP& P, const Place& w) {
+  if (w.vis <= 0) return 0;
+  if (P.ids) return (int)((((long long)P.take << P.R.lp) + TILE - 1) / TILE);
+  return (w.vis - start_of(w, P.shared) + TILE - 1) / TILE;
+}
+
+struct Seg { int row, head, t0, t1, nt; };   // tiles [t0, t1) of the nt tiles of (row, kv-head)
+
+template <int HD, int NT, bool BF>
+__global__ void __launch_bounds__(NT_, Lay<HD, NT>::CTAS)
+paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const AttnP P) {
+  using L = Lay<HD, NT>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t sb = s_u32(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t b_full = sb + L::OFF_BAR, b_empty = b_full + 8 * NSLOT, b_qfull = b_empty + 8 * NSLOT, b_qempty = b_qfull + 16;
+  volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::OFF_BAR + 16 * 8);
+  int* first = reinterpret_cast<int*>(smem + L::OFF_FIRST);
+  int* sums = reinterpret_cast<int*>(smem + L::OFF_SUM);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NSLOT; ++i) { bar_init(b_full + 8 * i, 1); bar_init(b_empty + 8 * i, CW); }
+    for (int i = 0; i < 2; ++i) { bar_init(b_qfull + 8 * i, 1); bar_init(b_qempty + 8 * i, CW); }
+    *s_abort = sb & 1023u ? 1 : 0;           // the swizzled tiles need a base of 1 KB
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pdl_wait();
+  pdl_launch();
+
+  // ---- the line: first[r] = tiles of one kv-head ahead of row r
+  {
+    constexpr int PER = ROWS / 128;
+    int n[PER], mine = 0, below = 0;
+    if (warp < CW) {
+      #pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int r = (int)threadIdx.x * PER + i;
+        n[i] = r < P.rows ? tiles_of(P, place_of(P.R, r)) : 0;
+        mine += n[i];
+      }
+      below = mine;
+      #pragma unroll
+      for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, below, d); if (lane >= d) below += o; }
+      if (lane == 31) sums[warp] = below;
+      below -= mine;
+    }
+    __syncthreads();
+    if (warp < CW) {
+      for (int i = 0; i < warp; ++i) below += sums[i];
+      #pragma unroll
+      for (int i = 0; i < PER; ++i) { first[threadIdx.x * PER + i] = below; below += n[i]; }
+      if (threadIdx.x == 127) first[ROWS] = below;
+    }
+    __syncthreads();
+  }
+  if (blockIdx.x == 0) for (int i = threadIdx.x; i <= P.rows; i += NT_) P.first[i] = first[i];          // for the merge
+  const int kvh = P.R.kvh, total = first[ROWS] * kvh, grid = min((int)gridDim.x, total), cta = (int)blockIdx.x;       // every CTA below `grid` has a tile at least
+  if (cta >= grid) return;
+  const int u0 = (int)((long long)total * cta / grid), u1 = (int)((long long)total * (cta + 1) / grid);
+
+  // The pair that holds unit u, and this CTA's part of it.
+  auto seg_at = [&](int u) {
+    int lo = 0, hi = P.rows - 1;             // last row whose first unit is not behind u
+    while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (first[mid] * kvh <= u) lo = mid; else hi = mid - 1; }
+    Seg s;
+    s.row = lo; s.nt = first[lo + 1] - first[lo];
+    const int in = u - first[lo] * kvh;
+    s.head = in / s.nt; s.t0 = in - s.head * s.nt;
+    s.t1 = min(s.nt, s.t0 + (u1 - u));
+    return s;
+  };
+  const int lc = min(P.R.lp, 6), chunk = 1 << lc, npt = TILE >> lc;    // rows of a box, boxes of a tile
+
+  if (warp == CW) {
+    // =========================================================================================== producer
+    const int none = (P.R.pages * kvh) << P.R.lp;                      // a row outside the arrays: zeros
+    int k = 0, sg = 0, issued = 0, queries = 0;                        // tiles and pairs so far; half stages and queries asked for
+    bool ok = *s_abort == 0;
+    for (int u = u0; u < u1 && ok; ++sg) {
+      const Seg s = seg_at(u);
+      u += s.t1 - s.t0;
+      const Place w = place_of(P.R, s.row);
+      const int start = start_of(w, P.shared);
+      // chunk ci of the pair: its row in the arrays, and the position of its first token (no token: INT_MAX)
+      auto chunk_at = [&](int ci, int& at, int& base) {
+        at = none; base = 0x7fffffff;
+        int b = -1, sub = 0;
+        if (P.ids) {
+          const int cpp = P.R.lp - lc, e = ci >> cpp;                  // log2 of a page's chunks; entry
+          if (e < P.take) b = P.ids[((size_t)s.row * kvh + s.head) * P.take + e];
+          sub = (ci & ((1 << cpp) - 1)) << lc;
+        } else {
+          const long long tok = start + ((long long)ci << lc);
+          if (tok < w.vis) { b = (int)(tok >> P.R.lp); sub = (int)tok & (P.R.page - 1); }
+        }
+        if (b < 0 || b >= P.R.blocks || ((long long)b << P.R.lp) + sub >= w.vis) return;
+        const int pg = page_of(P.R, w.seq, b);
+        if (pg < 0) return;
+        at = ((pg * kvh + s.head) << P.R.lp) + sub;
+        base = (b << P.R.lp) + sub;
+      };
+      // queries of the pair
+      if (sg >= 2 && !__all_sync(0xffffffffu, bar_wait(b_qempty + 8 * (sg & 1), ((sg >> 1) - 1) & 1))) { ok = false; break; }
+      if (lane == 0) bar_expect_tx(b_qfull + 8 * (sg & 1), P.g * HD * 2);
+      __syncwarp();
+      ++queries;
+      if (lane < P.g) bulk_1d(sb + L::OFF_Q + ((sg & 1) * NT * 8 + lane) * L::QP, P.q + s.row * P.qs + (size_t)(s.head * P.g + lane) * HD, HD * 2, b_qfull + 8 * (sg & 1));
+      int at0, base0, at1, base1;                                      // 32 chunks, and the 32 behind them, one a lane
+      const int tpb = 32 / npt;                                        // tiles of a batch
+      chunk_at(s.t0 * npt + lane, at0, base0);
+      chunk_at(s.t0 * npt + 32 + lane, at1, base1);
+      for (int t = s.t0; t < s.t1; ++t, ++k) {
+        int i = t - s.t0;
+        if (i > 0 && i % tpb == 0) { at0 = at1; base0 = base1; if (t + tpb < s.t1) chunk_at((t + tpb) * npt + lane, at1, base1); }
+        i = (i % tpb) * npt + (lane & (npt - 1));
+        const int at = __shfl_sync(0xffffffffu, at0, i), base = __shfl_sync(0xffffffffu, base0, i);
+        #pragma unroll
+        for (int v = 0; v < 2; ++v) {                                  // keys, values
+          const int it = 2 * k + v, slot = it % NSLOT;
+          if (it >= NSLOT && !__all_sync(0xffffffffu, bar_wait(b_empty + 8 * slot, (it / NSLOT - 1) & 1))) ok = false;
+          if (*s_abort) ok = false;
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (v == 0 && lane < npt) reinterpret_cast<int*>(smem + L::OFF_BASE)[(k % 3) * 4 + lane] = base;
+          __syncwarp();
+          if (lane == 0) bar_expect_tx(b_full + 8 * slot, L::HALF);    // whole boxes, rows outside the arrays among them
+          __syncwarp();
+          ++issued;
+          if (lane < npt) tma_3d(sb + slot * L::HALF + lane * (chunk * HD * 2), v ? &mapV : &mapK, 0, at, 0, b_full + 8 * slot);
+        }
+        if (!ok) break;
+      }
+    }
+    if (!ok) {                                                         // give up; the copies under way land before the block ends
+      if (lane == 0) { atomicExch(&g_attn_status, 7); *s_abort = 1; }
+      for (int it = max(0, issued - NSLOT); it < issued; ++it) bar_wait(b_full + 8 * (it % NSLOT), (it / NSLOT) & 1);
+      for (int it = max(0, queries - 2); it < queries; ++it) bar_wait(b_qfull + 8 * (it & 1), (it >> 1) & 1);
+    }
+    return;
+  }
+
+  // ============================================================================================= compute warps
+  const int g8 = lane >> 2, j = lane & 3;
+  const float cs = P.cs;
+  float* smax = reinterpret_cast<float*>(smem + L::OFF_MAX);
+  float* sl = reinterpret_cast<float*>(smem + L::OFF_L);
+  constexpr int MT = HD / CW / 16;                                     // 16-channel tiles of O of this warp
+  bool ok = true;
+  auto wait = [&](uint32_t bar, int n) {                               // phase n of a barrier
+    if (ok && !*s_abort && bar_wait(bar, n & 1)) return;
+    if (ok) { atomicExch(&g_attn_status, 7); *s_abort = 1; }
+    ok = false;
+  };
+  int k = 0, sg = 0;
+  for (int u = u0; u < u1; ++sg) {
+    const Seg s = seg_at(u);
+    u += s.t1 - s.t0;
+    const Place w = place_of(P.R, s.row);
+    uint32_t qf[NT][HD / 16][2];
+    wait(b_qfull + 8 * (sg & 1), sg >> 1);
+    #pragma unroll
+    for (int n = 0; n < NT; ++n)
+      #pragma unroll
+      for (int i = 0; i < HD / 32; ++i) {
+        uint32_t r[4];
+        ldm4(sb + L::OFF_Q + ((sg & 1) * NT * 8 + n * 8 + (lane & 7)) * L::QP + (4 * i + (lane >> 3)) * 16, r);
+        qf[n][2 * i][0] = r[0]; qf[n][2 * i][1] = r[1]; qf[n][2 * i + 1][0] = r[2]; qf[n][2 * i + 1][1] = r[3];
+      }
+    __syncwarp();
+    if (lane == 0) bar_arrive(b_qempty + 8 * (sg & 1));
+
+    float o[NT][MT][4], m[NT][2], l[NT][2];
+    #pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY; l[n][0] = l[n][1] = 0.f;
+      #pragma unroll
+      for (int x = 0; x < MT; ++x) o[n][x][0] = o[n][x][1] = o[n][x][2] = o[n][x][3] = 0.f;
+    }
+    for (int t = s.t0; t < s.t1; ++t, ++k) {
+      const int ik = 2 * k, kslot = ik % NSLOT, iv = ik + 1, vslot = iv % NSLOT, buf = k & 1;
+      // ---- S^T of this warp's 16 tokens
+      wait(b_full + 8 * kslot, ik / NSLOT);
+      const int tok = 16 * warp, cb = tok >> lc, rr = tok & (chunk - 1);                    // its chunk, first row there
+      const int4 b4 = *reinterpret_cast<const int4*>(smem + L::OFF_BASE + (k % 3) * 16);    // read before the half stage is handed back: the next tile's come then
+      auto base_of = [&](int i) { return i == 0 ? b4.x : i == 1 ? b4.y : i == 2 ? b4.z : b4.w; };
+      const int base = base_of(cb);
+      float c[NT][2][4];                                                                    // two sums, so that products do not wait for one another
+      #pragma unroll
+      for (int n = 0; n < NT; ++n)
+        #pragma unroll
+        for (int x = 0; x < 4; ++x) c[n][0][x] = c[n][1][x] = 0.f;
+      {
+        const int r = rr + (lane & 7) + ((lane >> 3) & 1) * 8;
+        const uint32_t a0 = sb + kslot * L::HALF + cb * (chunk * HD * 2) + r * 128;
+        #pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+          const int cc = 2 * ks + (lane >> 4);
+          uint32_t a[4];
+          ldm4(a0 + (cc >> 3) * (chunk * 128) + (((cc & 7) ^ (r & 7)) << 4), a);
+          #pragma unroll
+          for (int n = 0; n < NT; ++n) mma<BF>(c[n][ks & 1], a, qf[n][ks][0], qf[n][ks][1]);
+        }
+      }
+      // tokens of the tile that the row sees: lane row g8 and g8 + 8 of this warp's
+      const bool see0 = base != 0x7fffffff && base + rr + g8 < w.vis, see1 = base != 0x7fffffff && base + rr + g8 + 8 < w.vis;
+      float x[NT][4];
+      #pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) x[n][e] = (e < 2 ? see0 : see1) ? (c[n][0][e] + c[n][1][e]) * cs : -INFINITY;
+        #pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float v = fmaxf(x[n][e], x[n][e + 2]);
+          #pragma unroll
+          for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+          if (lane < 4) smax[(buf * CW + warp) * (NT * 8) + n * 8 + 2 * j + e] = v;
+        }
+      }
+      __syncwarp();
+      if (lane == 0) bar_arrive(b_empty + 8 * kslot);
+      compute_sync();
+      float alpha[NT][2];
+      #pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float2 top = make_float2(m[n][0], m[n][1]);
+        #pragma unroll
+        for (int i = 0; i < CW; ++i) {
+          const float2 f = *reinterpret_cast<const float2*>(smax + (buf * CW + i) * (NT * 8) + n * 8 + 2 * j);
+          top.x = fmaxf(top.x, f.x); top.y = fmaxf(top.y, f.y);
+        }
+        const float r0 = top.x == -INFINITY ? 0.f : top.x, r1 = top.y == -INFINITY ? 0.f : top.y;      // nothing seen so far: any reference does
+        alpha[n][0] = ex2(m[n][0] - r0); alpha[n][1] = ex2(m[n][1] - r1);
+        m[n][0] = top.x; m[n][1] = top.y;
+        const float p0 = ex2(x[n][0] - r0), p1 = ex2(x[n][1] - r1), p2 = ex2(x[n][2] - r0), p3 = ex2(x[n][3] - r1);
+        l[n][0] = l[n][0] * alpha[n][0] + (p0 + p2); l[n][1] = l[n][1] * alpha[n][1] + (p1 + p3);
+        stm2t(sb + L::OFF_P + (buf * NT * 8 + n * 8 + (lane & 7)) * L::PP + (tok + 8 * ((lane >> 3) & 1)) * 2, pack16<BF>(p0, p1), pack16<BF>(p2, p3));
+      }
+      // ---- O^T of this warp's channels
+      wait(b_full + 8 * vslot, iv / NSLOT);
+      const uint32_t sv = sb + vslot * L::HALF;
+      bool whole = true;                                                                    // every row of the tile is a token that the row sees, or came as zeros
+      for (int i = 0; i < npt; ++i) whole &= base_of(i) == 0x7fffffff || base_of(i) + chunk <= w.vis;
+      if (!whole) {
+        for (int i = threadIdx.x; i < TILE * (HD / 8); i += 128) {
+          const int r = i / (HD / 8), cc = i % (HD / 8), ch = r >> lc, rw = r & (chunk - 1);
+          if (base_of(ch) != 0x7fffffff && base_of(ch) + rw >= w.vis)
+            sts128(sv + ch * (chunk * HD * 2) + (cc >> 3) * (chunk * 128) + rw * 128 + (((cc & 7) ^ (rw & 7)) << 4), make_uint4(0u, 0u, 0u, 0u));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");                        // ahead of the copy that comes next into this half stage
+      }
+      compute_sync();
+      #pragma unroll
+      for (int n = 0; n < NT; ++n)
+        #pragma unroll
+        for (int y = 0; y < MT; ++y) { o[n][y][0] *= alpha[n][0]; o[n][y][1] *= alpha[n][1]; o[n][y][2] *= alpha[n][0]; o[n][y][3] *= alpha[n][1]; }
+      #pragma unroll
+      for (int h = 0; h < 2; ++h) {                                                         // 32 tokens
+        uint32_t pf[NT][4];
+        #pragma unroll
+        for (int n = 0; n < NT; ++n) ldm4(sb + L::OFF_P + (buf * NT * 8 + n * 8 + (lane & 7)) * L::PP + (4 * h + (lane >> 3)) * 16, pf[n]);
+        #pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          const int t16 = 32 * h + 16 * ks, ch = t16 >> lc, r = (t16 & (chunk - 1)) + (lane & 7) + ((lane >> 4) & 1) * 8;
+          #pragma unroll
+          for (int y = 0; y < MT; ++y) {
+            const int cc = warp * (2 * MT) + 2 * y + ((lane >> 3) & 1);
+            uint32_t a[4];
+            ldm4t(sv + ch * (chunk * HD * 2) + (cc >> 3) * (chunk * 128) + r * 128 + (((cc & 7) ^ (r & 7)) << 4), a);
+            #pragma unroll
+            for (int n = 0; n < NT; ++n) mma<BF>(o[n][y], a, pf[n][2 * ks], pf[n][2 * ks + 1]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) bar_arrive(b_empty + 8 * vslot);
+    }
+    // ---- this CTA's part of the pair
+    #pragma unroll
+    for (int n = 0; n < NT; ++n)
+      #pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        #pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+        if (lane < 4) sl[warp * (NT * 8) + n * 8 + 2 * j + e] = l[n][e];
+      }
+    compute_sync();
+    const bool direct = s.t1 - s.t0 == s.nt && start_of(w, P.shared) == 0;
+    const size_t piece = (size_t)cta + (size_t)s.row * kvh + s.head;
+    #pragma unroll
+    for (int n = 0; n < NT; ++n)
+      #pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int h = n * 8 + 2 * j + e;
+        float sum = 0.f;
+        #pragma unroll
+        for (int i = 0; i < CW; ++i) sum += sl[i * (NT * 8) + h];
+        if (h >= P.g || !ok) continue;
+        if (direct) {
+          uint16_t* dst = P.o16 + ((size_t)s.row * P.nh + s.head * P.g + h) * HD + warp * (HD / CW);
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;                                   // nothing seen: zeros
+          #pragma unroll
+          for (int y = 0; y < MT; ++y) {
+            const uint32_t v = pack16<BF>(sum == 0.f ? 0.f : o[n][y][e] * inv, sum == 0.f ? 0.f : o[n][y][e + 2] * inv);
+            dst[16 * y + g8] = (uint16_t)v; dst[16 * y + g8 + 8] = (uint16_t)(v >> 16);
+          }
+        } else {
+          float* dst = P.pacc + (piece * (NT * 8) + h) * HD + warp * (HD / CW);
+          #pragma unroll
+          for (int y = 0; y < MT; ++y) { dst[16 * y + g8] = o[n][y][e]; dst[16 * y + g8 + 8] = o[n][y][e + 2]; }
+          if (warp == 0 && g8 == 0) { P.pm[piece * (NT * 8) + h] = m[n][e]; P.pl[piece * (NT * 8) + h] = sum; }
+        }
+      }
+    compute_sync();                                                                         // the sums' places are free again
+  }
+}
+
+// Joins what the parts of a row hold: pieces of CTAs, and partials over the shared prefix.  A block takes `hpb` heads of a row, a head at a time: weights 2^(m - M) of
+// its parts in shared memory, then O, four channels a thread, the parts in THREADS * 4 / HD groups.
+constexpr int MERGE_THREADS = 256, MAX_PARTS = 2 * SMS + 64;
+template <int HD, bool BF>
+__global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnP P, int grid, int slot_rows, int hpb) {
+  constexpr int GROUPS = MERGE_THREADS * 4 / HD;
+  __shared__ float wgt[MAX_PARTS];
+  __shared__ float red[3][8];
+  __shared__ float4 part[GROUPS][HD / 4];
+  pdl_wait();
+  pdl_launch();
+  const int row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Place w = place_of(P.R, row);
+  if (w.seq < 0) return;
+  const int f0 = P.first[row], nt = P.first[row + 1] - f0, kvh = P.R.kvh;
+  const long long total = (long long)P.first[P.rows] * kvh;
+  grid = (int)min((long long)grid, total);
+  const bool prefix = start_of(w, P.shared) > 0;
+  const int np = prefix ? P.splits : 0;
+  for (int head = blockIdx.x * hpb; head < (int)(blockIdx.x + 1) * hpb; ++head) {
+    const int h = head / P.g, hh = head - h * P.g;
+    // CTAs [c0, c1] hold units [a, a + nt): CTA c begins at total * c / grid
+    const long long a = (long long)f0 * kvh + (long long)h * nt;
+    int c0 = 0, c1 = -1;
+    if (nt > 0) {
+      auto holder = [&](long long u) {       // the last CTA that begins at or ahead of u
+        int c = (int)(u * grid / total);
+        while (c + 1 < grid && total * (c + 1) / grid <= u) ++c;
+        while (c > 0 && total * c / grid > u) --c;
+        return c;
+      };
+      c0 = holder(a); c1 = holder(a + nt - 1);
+    }
+    if (!prefix && nt > 0 && c0 == c1) continue;                       // finished where it was computed
+    const int n = c1 - c0 + 1 + np;
+    const size_t pbase = (size_t)row * kvh + h;
+    auto m_at = [&](int i) { return i < np ? P.qm[((size_t)row * np + i) * P.nh + head] : P.pm[(c0 + (i - np) + pbase) * slot_rows + hh]; };
+    auto l_at = [&](int i) { return i < np ? P.ql[((size_t)row * np + i) * P.nh + head] : P.pl[(c0 + (i - np) + pbase) * slot_rows + hh]; };
+    float top = -INFINITY;
+    for (int i = threadIdx.x; i < n; i += MERGE_THREADS) if (l_at(i) != 0.f) top = fmaxf(top, m_at(i));
+    #pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if (lane == 0) red[0][warp] = top;
+    __syncthreads();
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, red[0][i]);
+    if (top == -INFINITY) top = 0.f;
+    float sum = 0.f;
+    for (int i = threadIdx.x; i < n; i += MERGE_THREADS) {
+      const float li = l_at(i), wi = li == 0.f ? 0.f : ex2(m_at(i) - top);
+      wgt[i] = wi; sum += li == 0.f ? 0.f : li * wi;
+    }
+    #pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) red[1][warp] = sum;
+    __syncthreads();
+    sum = 0.f;
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) sum += red[1][i];
+    const int grp = threadIdx.x / (HD / 4), ch = threadIdx.x % (HD / 4);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    #pragma unroll 4
+    for (int i = grp; i < n; i += GROUPS) {
+      const float* src = i < np ? P.qacc + (((size_t)row * np + i) * P.nh + head) * HD : P.pacc + ((c0 + (i - np) + pbase) * slot_rows + hh) * HD;
+      const float wi = wgt[i];
+      const float4 v = reinterpret_cast<const float4*>(src)[ch];
+      if (wi != 0.f) { acc.x += wi * v.x; acc.y += wi * v.y; acc.z += wi * v.z; acc.w += wi * v.w; }       // a part without weight may hold anything
+    }
+    part[grp][ch] = acc;
+    __syncthreads();
+    if (threadIdx.x < HD / 4) {
+      #pragma unroll
+      for (int i = 1; i < GROUPS; ++i) { const float4 v = part[i][ch]; acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w; }
+      const float inv = 1.f / sum;
+      uint2 y;
+      y.x = sum == 0.f ? 0u : pack16<BF>(acc.x * inv, acc.y * inv);
+      y.y = sum == 0.f ? 0u : pack16<BF>(acc.z * inv, acc.w * inv);
+      *reinterpret_cast<uint2*>(P.o16 + ((size_t)row * P.nh + head) * HD + 4 * ch) = y;
+    }
+    __syncthreads();
+  }
+}
+
+int ctas_of(int hd) { return SMS * (hd == 256 ? 1 : 2); }
+int slot_rows_of(int g) { return g <= 8 ? 8 : 16; }
+
+Work carve(void* ws, const yskn_paged_cache& c, int rows, int nh, int splits) {
+  const int chunk = std::min(rows, ROWS), sr = slot_rows_of(nh / c.kvh);
+  const size_t pieces = (size_t)ctas_of(c.hd) + (size_t)chunk * c.kvh, parts = (size_t)rows * splits * nh;
+  size_t at = 0;
+  auto take = [&](size_t n) { const size_t x = at; at = (at + n + 255) / 256 * 256; return static_cast<uint8_t*>(ws) + x; };
+  Work w;
+  w.first = reinterpret_cast<int*>(take((chunk + 1) * 4));
+  w.pm = reinterpret_cast<float*>(take(pieces * sr * 4));
+  w.pl = reinterpret_cast<float*>(take(pieces * sr * 4));
+  w.pacc = reinterpret_cast<float*>(take(pieces * sr * c.hd * 4));
+  w.qm = reinterpret_cast<float*>(take(parts * 4));
+  w.ql = reinterpret_cast<float*>(take(parts * 4));
+  w.qacc = reinterpret_cast<float*>(take(parts * c.hd * 4));
+  w.bytes = at;
+  return w;
+}
+
+template <int HD, int NT, bool BF>
+int launch(const yskn_paged_cache& c, const AttnP& P, cudaStream_t st) {
+  using L = Lay<HD, NT>;
+  auto kern = paged_attn_kernel<HD, NT, BF>;
+  static std::atomic<unsigned long long> attr{0};
+  if (first_use_on_device(attr)) KV4_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+  CUtensorMap mk, mv;
+  memcpy(&mk, c.maps[0], sizeof(mk)); memcpy(&mv, c.maps[1], sizeof(mv));
+  return launch_pdl("paged_attn_kernel", kern, dim3((unsigned)ctas_of(HD)), NT_, L::TOTAL, st, mk, mv, P);
+}
+template <int HD>
+int dispatch(const yskn_paged_cache& c, const AttnP& P, cudaStream_t st) {
+  const bool bf = c.dtype == YSKN_KV4_BF16;
+  if (P.g <= 8) return bf ? launch<HD, 1, true>(c, P, st) : launch<HD, 1, false>(c, P, st);
+  return bf ? launch<HD, 2, true>(c, P, st) : launch<HD, 2, false>(c, P, st);
+}
+
+}  // namespace
+
+int attn_status_fetch(int* out) {
+  int v = 0;
+  KV4_CUDA(cudaMemcpyFromSymbol(&v, g_attn_status, sizeof(int)));
+  const int zero = 0;
+  KV4_CUDA(cudaMemcpyToSymbol(g_attn_status, &zero, sizeof(int)));
+  *out = v; return 0;
+}
+
+}  // namespace paged
+
+size_t paged_attention_bytes(const yskn_paged_cache& c, int rows, int nh, int shared) {
+  const int splits = shared > 0 ? paged_prefix_splits(rows, nh / c.kvh, c.kvh, shared) : 0;
+  return paged::carve(nullptr, c, rows, nh, splits).bytes;
+}
+
+int launch_paged_attention(const yskn_paged_cache& c, const yskn_paged_rows& r, const yskn_paged_attn_args& a, cudaStream_t st) {
+  using namespace paged;
+  const int g = a.nh / c.kvh, splits = a.shared > 0 ? paged_prefix_splits(r.rows, g, c.kvh, a.shared) : 0;
+  const Work w = carve(a.workspace, c, r.rows, a.nh, splits);
+  if (splits > 0) if (int rc = launch_paged_prefix(c, r, a, splits, w, st)) return rc;
+  for (int first = 0; first < r.rows; first += ROWS) {
+    const int rows = std::min(ROWS, r.rows - first);
+    const size_t part = (size_t)first * splits * a.nh;
+    AttnP P{rows_of(c, r, first), rows, g, a.nh, static_cast<const uint16_t*>(a.q) + first * a.q_stride, (long long)a.q_stride, a.qscale * LOG2E,
+            static_cast<uint16_t*>(a.o16) + (size_t)first * a.nh * c.hd, splits > 0 ? a.shared : 0, a.ids ? a.ids + (size_t)first * c.kvh * a.take : nullptr, a.take,
+            w.first, w.pm, w.pl, w.pacc, w.qm + part, w.ql + part, w.qacc + part * c.hd, splits};
+    if (int rc = c.hd == 256 ? dispatch<256>(c, P, st) : dispatch<128>(c, P, st)) return rc;
+    // few rows: a block a head; many: a block a kv-head, since most of them have nothing to do
+    const int hpb = (long long)rows * a.nh <= 4 * 2 * SMS ? 1 : g;
+    auto merge = c.hd == 256 ? (c.dtype == YSKN_KV4_BF16 ? paged_merge_kernel<256, true> : paged_merge_kernel<256, false>)
+                             : (c.dtype == YSKN_KV4_BF16 ? paged_merge_kernel<128, true> : paged_merge_kernel<128, false>);
+    if (int rc = launch_pdl("paged_merge_kernel", merge, dim3((unsigned)(a.nh / hpb), (unsigned)rows), MERGE_THREADS, 0, st, P, ctas_of(c.hd), slot_rows_of(g), hpb)) return rc;
+  }
+  return 0;
+}
+
+}  // namespace kv4

@@ -1,0 +1,107 @@
+// Declarations shared by the kernels of the paged 16-bit cache (paged_append.cu, paged_select.cu, paged_attn.cu, paged_prefix.cu).
+#pragma once
+#include "kv4_common.cuh"
+#include <cuda.h>
+
+namespace kv4 {
+namespace paged {
+
+constexpr int SMS = 148;
+constexpr int TILE = 64;                     // tokens of one step of the attention kernel
+constexpr float LOG2E = 1.4426950408889634f;
+
+// What every kernel needs of the cache and of the call's rows.
+struct Rows {
+  const int* table; int seqs, blocks;        // page of block b of sequence s at table[s * blocks + b]
+  const int* seq; const int* pos;            // of each row
+  int pages, kvh, page, lp;                  // page = 1 << lp tokens
+};
+
+// A row's place: sequence, and how many tokens it sees.  seq < 0: the row is padding.
+struct Place { int seq, vis; };
+__device__ __forceinline__ Place place_of(const Rows& R, int row) {
+  const int s = R.seq[row], p = R.pos[row];
+  Place w;
+  w.seq = s >= 0 && s < R.seqs ? s : -1;
+  const long long cap = (long long)R.blocks << R.lp;
+  w.vis = w.seq < 0 || p < 0 ? 0 : (long long)p + 1 < cap ? p + 1 : (int)cap;
+  return w;
+}
+// Page of block b of sequence s; -1 where the table names none.
+__device__ __forceinline__ int page_of(const Rows& R, int s, int b) {
+  const int p = R.table[(size_t)s * R.blocks + b];
+  return p >= 0 && p < R.pages ? p : -1;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- PTX
+constexpr uint32_t WAIT_LIMIT = 1u << 22;    // polls before a wait gives up
+__device__ __forceinline__ uint32_t s_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void bar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {          // bounded; false = gave up
+  for (uint32_t i = 0; i < WAIT_LIMIT; ++i) if (bar_try(bar, parity)) return true;
+  return false;
+}
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(dst), "l"(m), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void bulk_1d(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+template <bool BF> __device__ __forceinline__ uint32_t pack16(float lo, float hi) {        // two values rounded to the 16-bit type
+  uint32_t d;
+  if (BF) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+template <bool BF> __device__ __forceinline__ float2 unpack16(uint32_t w) {
+  if (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  const __half2 h = *reinterpret_cast<const __half2*>(&w);
+  return __half22float2(h);
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v; asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory"); return v;
+}
+__device__ __forceinline__ void sts128(uint32_t a, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// Workspace of one attention call.  Pieces of rows that lie on several CTAs: (m, l) and O of the heads of a kv-head; partials over the shared
+// prefix, in the layout [row][split][head]; the first tile of every row.
+struct Work {
+  int* first; float* pm; float* pl; float* pacc; float* qm; float* ql; float* qacc;
+  size_t bytes;
+};
+
+}  // namespace paged
+
+int launch_paged_append(const yskn_paged_cache& c, const yskn_paged_rows& r, const yskn_paged_append_args& a, cudaStream_t st);
+int launch_paged_select(const yskn_paged_cache& c, const yskn_paged_rows& r, const yskn_paged_select_args& a, cudaStream_t st);
+int launch_paged_attention(const yskn_paged_cache& c, const yskn_paged_rows& r, const yskn_paged_attn_args& a, cudaStream_t st);
+size_t paged_attention_bytes(const yskn_paged_cache& c, int rows, int nh, int shared);
+size_t paged_select_bytes(const yskn_paged_cache& c, int rows, int blocks);
+int paged_prefix_splits(int rows, int g, int kvh, int shared);
+int launch_paged_prefix(const yskn_paged_cache& c, const yskn_paged_rows& r, const yskn_paged_attn_args& a, int splits, const paged::Work& w, cudaStream_t st);
+
+namespace paged {
+inline Rows rows_of(const yskn_paged_cache& c, const yskn_paged_rows& r, int first) {
+  int lp = 0;
+  while ((1 << lp) < c.page) ++lp;
+  return Rows{r.table, r.seqs, r.blocks, r.seq + first, r.pos + first, c.pages, c.kvh, c.page, lp};
+}
+}  // namespace paged
+}  // namespace kv4
