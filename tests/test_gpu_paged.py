@@ -165,6 +165,54 @@ def test_values_that_are_not_finite_stay_in_their_channel():
     assert torch.isinf(o16[0, :, 17]).all() and torch.isfinite(o16[0, :, :17]).all() and torch.isfinite(o16[0, :, 18:]).all()
 
 
+# ---------------------------------------------------------------------------------------------------------------- a shared part
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("nh,hkv,hd,page,shared,behind", [
+    (24, 4, 256, 64, 64, [0]),                                   # a row that ends with the shared part
+    (24, 4, 256, 64, 1024, [1, 70, 64]),
+    (28, 4, 128, 16, 16, [5, 0, 300, 16]),                       # less than a tile of keys
+    (28, 4, 128, 32, 992, [(7 * i) % 90 for i in range(40)]),
+    (16, 2, 128, 128, 4096, [1 + i for i in range(20)]),
+    (32, 2, 256, 16, 400, [3] * 9),
+    (4, 4, 128, 64, 8192, [(3 * i) % 5 for i in range(130)]),    # one head a kv-head, more rows than a tile holds
+    (24, 4, 256, 32, 2592, [(11 * i) % 40 for i in range(50)]),
+])
+def test_rows_behind_a_shared_part(dt, nh, hkv, hd, page, shared, behind):
+    lengths = [shared + n for n in behind]
+    k, v, table, g = make_pool(lengths, hkv, hd, page, DT[dt], seed=shared + len(behind), garbage=True, shared=shared)
+    n = len(lengths)
+    q = torch.randn((n, nh, hd), generator=g, device="cuda").to(DT[dt])
+    seq, pos = torch.arange(n, dtype=torch.int32, device="cuda"), ints(lengths) - 1
+    o16, before = attend(k, v, table, seq, pos, q, hd ** -0.5, shared=shared)
+    some = list(range(n)) if n <= 40 else list(range(0, n, 5)) + [n - 1]
+    check_rows(o16[some], q[some], k, v, table, seq[some], pos[some], hd ** -0.5, before=before[some])
+
+
+def test_shared_part_with_short_and_padding_rows():
+    """Rows shorter than the shared part attend by themselves; padding rows and rows that see nothing stay what they are, the first ones too."""
+    shared, lengths = 640, [700, 640, 641, 900]
+    k, v, table, g = make_pool(lengths, 4, 128, 64, torch.bfloat16, seed=8, garbage=True, shared=shared)
+    seq, pos = ints([-1, 0, 0, 1, 2, 3, 3, 3, 9, 1]), ints([699, -1, 300, 639, 640, 899, 638, 0, 640, -7])
+    q = torch.randn((10, 28, 128), generator=g, device="cuda").bfloat16()
+    for scale in (0.09, -0.09):
+        o16, before = attend(k, v, table, seq, pos, q, scale, shared=shared)
+        check_rows(o16, q, k, v, table, seq, pos, scale, before=before)
+    pos[:] = -1                                                  # no row at all has the shared part
+    o16, before = attend(k, v, table, seq, pos, q, 0.09, shared=shared)
+    check_rows(o16, q, k, v, table, seq, pos, 0.09, before=before)
+
+
+def test_shared_part_with_large_scores_and_rising_maxima():
+    """The running maximum grows from tile to tile by more than the rescale's margin."""
+    shared = 2048
+    k, v, table, g = make_pool([shared + 10, shared + 3], 2, 128, 64, torch.float16, seed=6, shared=shared)
+    for b in range(shared // 64):
+        k[int(table[0, b])] *= 0.1 * (b + 1)
+    q = torch.randn((2, 16, 128), generator=g, device="cuda").half() * 8
+    o16, before = attend(k, v, table, ints([0, 1]), ints([shared + 9, shared + 2]), q, 0.2, shared=shared)
+    check_rows(o16, q, k, v, table, [0, 1], [shared + 9, shared + 2], 0.2, before=before)
+
+
 # ---------------------------------------------------------------------------------------------------------------- chosen blocks
 @pytest.mark.parametrize("dt", ["f16", "bf16"])
 @pytest.mark.parametrize("nh,hkv,hd,page,lengths,take", [
