@@ -29,7 +29,7 @@ __device__ int g_attn_status = 0;            // 0 ok; 7 = a bounded wait ran out
 
 namespace {
 
-constexpr int ROWS = 512;                    // rows of one launch
+constexpr int ROWS = 256;                    // rows of one launch
 constexpr int NSLOT = 6;                     // half stages of the ring: K, V, K, V, K, V
 constexpr int CW = 4, NT_ = (CW + 1) * 32;   // compute warps; threads
 
@@ -38,14 +38,14 @@ struct AttnP {
   const uint16_t* q; long long qs; float cs; // cs = qscale * log2(e)
   uint16_t* o16;
   int shared; const int* ids; int take;
-  int* first; float* pm; float* pl; float* pacc;       // pieces
-  const float* qm; const float* ql; const float* qacc; int splits;     // partials over the shared prefix
+  int2* span; float2* ml; float* pacc;       // first and last CTA of a pair; its pieces: maxima and sums, O
+  const float2* qml; const float* qacc; int splits;     // partials over the shared prefix
 };
 
 template <int HD, int NT> struct Lay {
   static constexpr int HALF = TILE * HD * 2, QP = HD * 2 + 16, PP = TILE * 2 + 16;   // bytes: a half stage; a row of Q; a row of P (paddings: eight rows on different banks)
   static constexpr int OFF_Q = NSLOT * HALF, OFF_P = OFF_Q + 2 * NT * 8 * QP, OFF_MAX = OFF_P + 2 * NT * 8 * PP, OFF_L = OFF_MAX + 2 * CW * NT * 8 * 4;
-  static constexpr int OFF_BASE = OFF_L + CW * NT * 8 * 4, OFF_BAR = OFF_BASE + 3 * 4 * 4, OFF_SUM = OFF_BAR + 16 * 8 + 8, OFF_FIRST = OFF_SUM + 32;
+  static constexpr int OFF_BASE = OFF_L + CW * NT * 8 * 4, OFF_BAR = OFF_BASE + 3 * 4 * 4, OFF_SUM = OFF_BAR + 16 * 8 + 8, OFF_PLACE = OFF_SUM + 32, OFF_FIRST = OFF_PLACE + ROWS * 8;
   static constexpr int TOTAL = OFF_FIRST + (ROWS + 1) * 4;
   static constexpr int CTAS = HD == 256 ? 1 : 2;
   static_assert(HALF % 1024 == 0 && OFF_BASE % 16 == 0 && OFF_BAR % 8 == 0 && CTAS * (TOTAL + 1024) <= 228 * 1024, "shared memory");
@@ -76,8 +76,6 @@ __device__ __forceinline__ int tiles_of(const AttnP& P, const Place& w) {
   return (w.vis - start_of(w, P.shared) + TILE - 1) / TILE;
 }
 
-struct Seg { int row, head, t0, t1, nt; };   // tiles [t0, t1) of the nt tiles of (row, kv-head)
-
 template <int HD, int NT, bool BF>
 __global__ void __launch_bounds__(NT_, Lay<HD, NT>::CTAS)
 paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const AttnP P) {
@@ -89,6 +87,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
   volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::OFF_BAR + 16 * 8);
   int* first = reinterpret_cast<int*>(smem + L::OFF_FIRST);
   int* sums = reinterpret_cast<int*>(smem + L::OFF_SUM);
+  Place* places = reinterpret_cast<Place*>(smem + L::OFF_PLACE);
   if (threadIdx.x == 0) {
     for (int i = 0; i < NSLOT; ++i) { bar_init(b_full + 8 * i, 1); bar_init(b_empty + 8 * i, CW); }
     for (int i = 0; i < 2; ++i) { bar_init(b_qfull + 8 * i, 1); bar_init(b_qempty + 8 * i, CW); }
@@ -106,7 +105,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
       #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int r = (int)threadIdx.x * PER + i;
-        n[i] = r < P.rows ? tiles_of(P, place_of(P.R, r)) : 0;
+        n[i] = 0;
+        if (r < P.rows) { const Place w = place_of(P.R, r); places[r] = w; n[i] = tiles_of(P, w); }
         mine += n[i];
       }
       below = mine;
@@ -124,82 +124,79 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     }
     __syncthreads();
   }
-  if (blockIdx.x == 0) for (int i = threadIdx.x; i <= P.rows; i += NT_) P.first[i] = first[i];          // for the merge
   const int kvh = P.R.kvh, total = first[ROWS] * kvh, grid = min((int)gridDim.x, total), cta = (int)blockIdx.x;       // every CTA below `grid` has a tile at least
   if (cta >= grid) return;
   const int u0 = (int)((long long)total * cta / grid), u1 = (int)((long long)total * (cta + 1) / grid);
 
-  // The pair that holds unit u, and this CTA's part of it.
-  auto seg_at = [&](int u) {
-    int lo = 0, hi = P.rows - 1;             // last row whose first unit is not behind u
+  // The row that holds unit u: the last whose first unit is not behind it
+  auto row_of = [&](int u) {
+    int lo = 0, hi = P.rows - 1;
     while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (first[mid] * kvh <= u) lo = mid; else hi = mid - 1; }
-    Seg s;
-    s.row = lo; s.nt = first[lo + 1] - first[lo];
-    const int in = u - first[lo] * kvh;
-    s.head = in / s.nt; s.t0 = in - s.head * s.nt;
-    s.t1 = min(s.nt, s.t0 + (u1 - u));
-    return s;
+    return lo;
   };
   const int lc = min(P.R.lp, 6), chunk = 1 << lc, npt = TILE >> lc;    // rows of a box, boxes of a tile
 
   if (warp == CW) {
     // =========================================================================================== producer
     const int none = (P.R.pages * kvh) << P.R.lp;                      // a row outside the arrays: zeros
-    int k = 0, sg = 0, issued = 0, queries = 0;                        // tiles and pairs so far; half stages and queries asked for
+    // Boxes come 32 at a time, one a lane, looked up a batch ahead and across the borders of pairs: the lookups' latency (place, chosen block, table) is never
+    // waited for.  A box: its row in the arrays, the position of its first token (no token: INT_MAX), its pair.
+    struct Box { int at, base, pair; };
+    auto box_of = [&](int u, int j) {                                  // box j of unit u
+      Box x{none, 0x7fffffff, -1};
+      if (u >= u1) return x;
+      const int row = row_of(u), nt = first[row + 1] - first[row], in = u - first[row] * kvh, head = in / nt;
+      const Place w = places[row];
+      x.pair = row * kvh + head;
+      const int ci = (in - head * nt) * npt + j;
+      int b = -1, sub = 0;
+      if (P.ids) {
+        const int cpp = P.R.lp - lc, e = ci >> cpp;                    // log2 of a page's boxes; entry
+        if (e < P.take) b = P.ids[(size_t)x.pair * P.take + e];
+        sub = (ci & ((1 << cpp) - 1)) << lc;
+      } else {
+        const long long tok = start_of(w, P.shared) + ((long long)ci << lc);
+        if (tok < w.vis) { b = (int)(tok >> P.R.lp); sub = (int)tok & (P.R.page - 1); }
+      }
+      if (b < 0 || b >= P.R.blocks || ((long long)b << P.R.lp) + sub >= w.vis) return x;
+      const int pg = page_of(P.R, w.seq, b);
+      if (pg < 0) return x;
+      x.at = ((pg * kvh + head) << P.R.lp) + sub;
+      x.base = (b << P.R.lp) + sub;
+      return x;
+    };
+    int k = 0, pair = -1, issued = 0, queries = 0;                     // tiles so far; the pair they belong to; half stages and queries asked for
     bool ok = *s_abort == 0;
-    for (int u = u0; u < u1 && ok; ++sg) {
-      const Seg s = seg_at(u);
-      u += s.t1 - s.t0;
-      const Place w = place_of(P.R, s.row);
-      const int start = start_of(w, P.shared);
-      // chunk ci of the pair: its row in the arrays, and the position of its first token (no token: INT_MAX)
-      auto chunk_at = [&](int ci, int& at, int& base) {
-        at = none; base = 0x7fffffff;
-        int b = -1, sub = 0;
-        if (P.ids) {
-          const int cpp = P.R.lp - lc, e = ci >> cpp;                  // log2 of a page's chunks; entry
-          if (e < P.take) b = P.ids[((size_t)s.row * kvh + s.head) * P.take + e];
-          sub = (ci & ((1 << cpp) - 1)) << lc;
-        } else {
-          const long long tok = start + ((long long)ci << lc);
-          if (tok < w.vis) { b = (int)(tok >> P.R.lp); sub = (int)tok & (P.R.page - 1); }
-        }
-        if (b < 0 || b >= P.R.blocks || ((long long)b << P.R.lp) + sub >= w.vis) return;
-        const int pg = page_of(P.R, w.seq, b);
-        if (pg < 0) return;
-        at = ((pg * kvh + s.head) << P.R.lp) + sub;
-        base = (b << P.R.lp) + sub;
-      };
-      // queries of the pair
-      if (sg >= 2 && !__all_sync(0xffffffffu, bar_wait(b_qempty + 8 * (sg & 1), ((sg >> 1) - 1) & 1))) { ok = false; break; }
-      if (lane == 0) bar_expect_tx(b_qfull + 8 * (sg & 1), P.g * HD * 2);
-      __syncwarp();
-      ++queries;
-      if (lane < P.g) bulk_1d(sb + L::OFF_Q + ((sg & 1) * NT * 8 + lane) * L::QP, P.q + s.row * P.qs + (size_t)(s.head * P.g + lane) * HD, HD * 2, b_qfull + 8 * (sg & 1));
-      int at0, base0, at1, base1;                                      // 32 chunks, and the 32 behind them, one a lane
-      const int tpb = 32 / npt;                                        // tiles of a batch
-      chunk_at(s.t0 * npt + lane, at0, base0);
-      chunk_at(s.t0 * npt + 32 + lane, at1, base1);
-      for (int t = s.t0; t < s.t1; ++t, ++k) {
-        int i = t - s.t0;
-        if (i > 0 && i % tpb == 0) { at0 = at1; base0 = base1; if (t + tpb < s.t1) chunk_at((t + tpb) * npt + lane, at1, base1); }
-        i = (i % tpb) * npt + (lane & (npt - 1));
-        const int at = __shfl_sync(0xffffffffu, at0, i), base = __shfl_sync(0xffffffffu, base0, i);
-        #pragma unroll
-        for (int v = 0; v < 2; ++v) {                                  // keys, values
-          const int it = 2 * k + v, slot = it % NSLOT;
-          if (it >= NSLOT && !__all_sync(0xffffffffu, bar_wait(b_empty + 8 * slot, (it / NSLOT - 1) & 1))) ok = false;
-          if (*s_abort) ok = false;
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          if (v == 0 && lane < npt) reinterpret_cast<int*>(smem + L::OFF_BASE)[(k % 3) * 4 + lane] = base;
-          __syncwarp();
-          if (lane == 0) bar_expect_tx(b_full + 8 * slot, L::HALF);    // whole boxes, rows outside the arrays among them
-          __syncwarp();
-          ++issued;
-          if (lane < npt) tma_3d(sb + slot * L::HALF + lane * (chunk * HD * 2), v ? &mapV : &mapK, 0, at, 0, b_full + 8 * slot);
-        }
+    const int tpb = 32 / npt, jl = lane & (npt - 1), tl = lane / npt;  // tiles of a batch; this lane's box and tile in it
+    Box now = box_of(u0 + tl, jl), next = box_of(u0 + tpb + tl, jl);
+    for (int u = u0; u < u1 && ok; ++u, ++k) {
+      int i = u - u0;
+      if (i > 0 && i % tpb == 0) { now = next; next = box_of(u + tpb + tl, jl); }
+      i = (i % tpb) * npt + jl;
+      const int at = __shfl_sync(0xffffffffu, now.at, i), base = __shfl_sync(0xffffffffu, now.base, i), pr = __shfl_sync(0xffffffffu, now.pair, i);
+      if (pr != pair) {                                                // queries of the next pair
+        pair = pr;
+        const int sg = queries;
+        if (sg >= 2 && !__all_sync(0xffffffffu, bar_wait(b_qempty + 8 * (sg & 1), ((sg >> 1) - 1) & 1))) { ok = false; break; }
+        if (lane == 0) bar_expect_tx(b_qfull + 8 * (sg & 1), P.g * HD * 2);
+        __syncwarp();
+        ++queries;
+        const int row = pair / kvh, head = pair - row * kvh;
+        if (lane < P.g) bulk_1d(sb + L::OFF_Q + ((sg & 1) * NT * 8 + lane) * L::QP, P.q + row * P.qs + (size_t)(head * P.g + lane) * HD, HD * 2, b_qfull + 8 * (sg & 1));
+      }
+      #pragma unroll
+      for (int v = 0; v < 2; ++v) {                                    // keys, values
+        const int it = 2 * k + v, slot = it % NSLOT;
+        if (it >= NSLOT && !__all_sync(0xffffffffu, bar_wait(b_empty + 8 * slot, (it / NSLOT - 1) & 1))) ok = false;
+        if (*s_abort) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
+        if (v == 0 && lane < npt) reinterpret_cast<int*>(smem + L::OFF_BASE)[(k % 3) * 4 + lane] = base;
+        __syncwarp();
+        if (lane == 0) bar_expect_tx(b_full + 8 * slot, L::HALF);      // whole boxes, rows outside the arrays among them
+        __syncwarp();
+        ++issued;
+        if (lane < npt) tma_3d(sb + slot * L::HALF + lane * (chunk * HD * 2), v ? &mapV : &mapK, 0, at, 0, b_full + 8 * slot);
       }
     }
     if (!ok) {                                                         // give up; the copies under way land before the block ends
@@ -222,11 +219,11 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     if (ok) { atomicExch(&g_attn_status, 7); *s_abort = 1; }
     ok = false;
   };
-  int k = 0, sg = 0;
-  for (int u = u0; u < u1; ++sg) {
-    const Seg s = seg_at(u);
-    u += s.t1 - s.t0;
-    const Place w = place_of(P.R, s.row);
+  int k = 0, sg = 0, row = row_of(u0), nt = first[row + 1] - first[row], head = (u0 - first[row] * kvh) / nt, t0 = u0 - first[row] * kvh - head * nt;
+  for (int u = u0; u < u1; ++sg) {                                     // tiles [t0, t1) of the nt tiles of (row, kv-head)
+    const int t1 = min(nt, t0 + (u1 - u));
+    u += t1 - t0;
+    const Place w = places[row];
     uint32_t qf[NT][HD / 16][2];
     wait(b_qfull + 8 * (sg & 1), sg >> 1);
     #pragma unroll
@@ -247,7 +244,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
       #pragma unroll
       for (int x = 0; x < MT; ++x) o[n][x][0] = o[n][x][1] = o[n][x][2] = o[n][x][3] = 0.f;
     }
-    for (int t = s.t0; t < s.t1; ++t, ++k) {
+    for (int t = t0; t < t1; ++t, ++k) {
       const int ik = 2 * k, kslot = ik % NSLOT, iv = ik + 1, vslot = iv % NSLOT, buf = k & 1;
       // ---- S^T of this warp's 16 tokens
       wait(b_full + 8 * kslot, ik / NSLOT);
@@ -355,8 +352,10 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
         if (lane < 4) sl[warp * (NT * 8) + n * 8 + 2 * j + e] = l[n][e];
       }
     compute_sync();
-    const bool direct = s.t1 - s.t0 == s.nt && start_of(w, P.shared) == 0;
-    const size_t piece = (size_t)cta + (size_t)s.row * kvh + s.head;
+    const bool direct = t1 - t0 == nt && start_of(w, P.shared) == 0;
+    const int pair = row * kvh + head;
+    const size_t piece = (size_t)cta + pair;
+    if (threadIdx.x == 0) { if (t0 == 0) P.span[pair].x = cta; if (t1 == nt) P.span[pair].y = cta; }
     #pragma unroll
     for (int n = 0; n < NT; ++n)
       #pragma unroll
@@ -367,7 +366,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
         for (int i = 0; i < CW; ++i) sum += sl[i * (NT * 8) + h];
         if (h >= P.g || !ok) continue;
         if (direct) {
-          uint16_t* dst = P.o16 + ((size_t)s.row * P.nh + s.head * P.g + h) * HD + warp * (HD / CW);
+          uint16_t* dst = P.o16 + ((size_t)row * P.nh + head * P.g + h) * HD + warp * (HD / CW);
           const float inv = sum == 0.f ? 0.f : 1.f / sum;                                   // nothing seen: zeros
           #pragma unroll
           for (int y = 0; y < MT; ++y) {
@@ -378,94 +377,87 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
           float* dst = P.pacc + (piece * (NT * 8) + h) * HD + warp * (HD / CW);
           #pragma unroll
           for (int y = 0; y < MT; ++y) { dst[16 * y + g8] = o[n][y][e]; dst[16 * y + g8 + 8] = o[n][y][e + 2]; }
-          if (warp == 0 && g8 == 0) { P.pm[piece * (NT * 8) + h] = m[n][e]; P.pl[piece * (NT * 8) + h] = sum; }
+          if (warp == 0 && g8 == 0) P.ml[piece * (NT * 8) + h] = make_float2(m[n][e], sum);
         }
       }
     compute_sync();                                                                         // the sums' places are free again
+    t0 = 0;
+    if (++head == kvh) { head = 0; do ++row; while (row < P.rows && first[row + 1] == first[row]); nt = row < P.rows ? first[row + 1] - first[row] : 1; }
   }
 }
 
-// Joins what the parts of a row hold: pieces of CTAs, and partials over the shared prefix.  A block takes `hpb` heads of a row, a head at a time: weights 2^(m - M) of
-// its parts in shared memory, then O, four channels a thread, the parts in THREADS * 4 / HD groups.
-constexpr int MERGE_THREADS = 256, MAX_PARTS = 2 * SMS + 64;
-template <int HD, bool BF>
-__global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnP P, int grid, int slot_rows, int hpb) {
-  constexpr int GROUPS = MERGE_THREADS * 4 / HD;
-  __shared__ float wgt[MAX_PARTS];
-  __shared__ float red[3][8];
-  __shared__ float4 part[GROUPS][HD / 4];
+// Joins what the parts of a (row, head) hold: partials over the shared prefix, then pieces of CTAs.  W warps a (row, head): each looks at all parts' maxima and sums by itself,
+// a lane a part, and adds up every W-th part's O, HD / 32 channels a lane.
+constexpr int MERGE_THREADS = 256;
+template <int HD, bool BF, int W>
+__global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnP P, int slot_rows) {
+  constexpr int V = HD / 128;                // float4 of a lane
+  __shared__ float4 part[W > 1 ? W : 1][W > 1 ? HD / 4 : 1];
   pdl_wait();
   pdl_launch();
-  const int row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, wid = (int)(blockIdx.x * (MERGE_THREADS / 32) + (threadIdx.x >> 5)), x = wid / W, wi = wid % W;
+  if (x >= P.rows * P.nh) return;            // the same for the whole block where W is its number of warps
+  const int row = x / P.nh, head = x - row * P.nh, h = head / P.g, hh = head - h * P.g, pair = row * P.R.kvh + h;
+  const int2 span = P.span[pair];            // of a row without tiles nobody has written it, and nobody looks at it
   const Place w = place_of(P.R, row);
   if (w.seq < 0) return;
-  const int f0 = P.first[row], nt = P.first[row + 1] - f0, kvh = P.R.kvh;
-  const long long total = (long long)P.first[P.rows] * kvh;
-  grid = (int)min((long long)grid, total);
-  const bool prefix = start_of(w, P.shared) > 0;
-  const int np = prefix ? P.splits : 0;
-  for (int head = blockIdx.x * hpb; head < (int)(blockIdx.x + 1) * hpb; ++head) {
-    const int h = head / P.g, hh = head - h * P.g;
-    // CTAs [c0, c1] hold units [a, a + nt): CTA c begins at total * c / grid
-    const long long a = (long long)f0 * kvh + (long long)h * nt;
-    int c0 = 0, c1 = -1;
-    if (nt > 0) {
-      auto holder = [&](long long u) {       // the last CTA that begins at or ahead of u
-        int c = (int)(u * grid / total);
-        while (c + 1 < grid && total * (c + 1) / grid <= u) ++c;
-        while (c > 0 && total * c / grid > u) --c;
-        return c;
-      };
-      c0 = holder(a); c1 = holder(a + nt - 1);
-    }
-    if (!prefix && nt > 0 && c0 == c1) continue;                       // finished where it was computed
-    const int n = c1 - c0 + 1 + np;
-    const size_t pbase = (size_t)row * kvh + h;
-    auto m_at = [&](int i) { return i < np ? P.qm[((size_t)row * np + i) * P.nh + head] : P.pm[(c0 + (i - np) + pbase) * slot_rows + hh]; };
-    auto l_at = [&](int i) { return i < np ? P.ql[((size_t)row * np + i) * P.nh + head] : P.pl[(c0 + (i - np) + pbase) * slot_rows + hh]; };
-    float top = -INFINITY;
-    for (int i = threadIdx.x; i < n; i += MERGE_THREADS) if (l_at(i) != 0.f) top = fmaxf(top, m_at(i));
-    #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if (lane == 0) red[0][warp] = top;
-    __syncthreads();
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, red[0][i]);
-    if (top == -INFINITY) top = 0.f;
-    float sum = 0.f;
-    for (int i = threadIdx.x; i < n; i += MERGE_THREADS) {
-      const float li = l_at(i), wi = li == 0.f ? 0.f : ex2(m_at(i) - top);
-      wgt[i] = wi; sum += li == 0.f ? 0.f : li * wi;
-    }
-    #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) red[1][warp] = sum;
-    __syncthreads();
-    sum = 0.f;
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) sum += red[1][i];
-    const int grp = threadIdx.x / (HD / 4), ch = threadIdx.x % (HD / 4);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const bool prefix = start_of(w, P.shared) > 0, own = tiles_of(P, w) > 0;
+  if (!prefix && own && span.x == span.y) return;                      // finished where it was computed
+  const int np = prefix ? P.splits : 0, n = np + (own ? span.y - span.x + 1 : 0);
+  const float2* qml = P.qml + (size_t)row * P.splits * P.nh + head;
+  const float* qacc = P.qacc + ((size_t)row * P.splits * P.nh + head) * HD;
+  const size_t piece0 = ((size_t)span.x + pair) * slot_rows + hh;      // piece c of the pair: + c * slot_rows
+  auto ml_at = [&](int i) { return i < np ? qml[(size_t)i * P.nh] : P.ml[piece0 + (size_t)(i - np) * slot_rows]; };
+  auto o_at = [&](int i) { return i < np ? qacc + (size_t)i * P.nh * HD : P.pacc + (piece0 + (size_t)(i - np) * slot_rows) * HD; };
+  float top = -INFINITY;
+  for (int i = lane; i < n; i += 32) { const float2 f = ml_at(i); if (f.y != 0.f) top = fmaxf(top, f.x); }
+  #pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  if (top == -INFINITY) top = 0.f;
+  float sum = 0.f;
+  float4 acc[V];
+  #pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    float wt = 0.f;
+    if (i0 + lane < n) { const float2 f = ml_at(i0 + lane); if (f.y != 0.f) { wt = ex2(f.x - top); sum += f.y * wt; } }
+    const int m = min(32, n - i0);
     #pragma unroll 4
-    for (int i = grp; i < n; i += GROUPS) {
-      const float* src = i < np ? P.qacc + (((size_t)row * np + i) * P.nh + head) * HD : P.pacc + ((c0 + (i - np) + pbase) * slot_rows + hh) * HD;
-      const float wi = wgt[i];
-      const float4 v = reinterpret_cast<const float4*>(src)[ch];
-      if (wi != 0.f) { acc.x += wi * v.x; acc.y += wi * v.y; acc.z += wi * v.z; acc.w += wi * v.w; }       // a part without weight may hold anything
-    }
-    part[grp][ch] = acc;
-    __syncthreads();
-    if (threadIdx.x < HD / 4) {
+    for (int k = wi; k < m; k += W) {
+      const float wk = __shfl_sync(0xffffffffu, wt, k);
+      const float4* src = reinterpret_cast<const float4*>(o_at(i0 + k)) + lane;
       #pragma unroll
-      for (int i = 1; i < GROUPS; ++i) { const float4 v = part[i][ch]; acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w; }
-      const float inv = 1.f / sum;
-      uint2 y;
-      y.x = sum == 0.f ? 0u : pack16<BF>(acc.x * inv, acc.y * inv);
-      y.y = sum == 0.f ? 0u : pack16<BF>(acc.z * inv, acc.w * inv);
-      *reinterpret_cast<uint2*>(P.o16 + ((size_t)row * P.nh + head) * HD + 4 * ch) = y;
+      for (int v = 0; v < V; ++v) {
+        const float4 f = src[32 * v];
+        if (wk != 0.f) { acc[v].x += wk * f.x; acc[v].y += wk * f.y; acc[v].z += wk * f.z; acc[v].w += wk * f.w; }      // a part without weight may hold anything
+      }
     }
-    __syncthreads();
   }
+  #pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (W > 1) {
+    #pragma unroll
+    for (int v = 0; v < V; ++v) part[W > 1 ? wi : 0][W > 1 ? 32 * v + lane : 0] = acc[v];
+    __syncthreads();
+    if (wi >= V) return;                     // warp v finishes channels 128 v .. 128 v + 127
+    acc[0] = make_float4(0.f, 0.f, 0.f, 0.f);
+    #pragma unroll
+    for (int i = 0; i < W; ++i) { const float4 f = part[W > 1 ? i : 0][W > 1 ? 32 * wi + lane : 0]; acc[0].x += f.x; acc[0].y += f.y; acc[0].z += f.z; acc[0].w += f.w; }
+  }
+  const float inv = 1.f / sum;
+  #pragma unroll
+  for (int v = 0; v < (W > 1 ? 1 : V); ++v) {
+    uint2 y;
+    y.x = sum == 0.f ? 0u : pack16<BF>(acc[v].x * inv, acc[v].y * inv);
+    y.y = sum == 0.f ? 0u : pack16<BF>(acc[v].z * inv, acc[v].w * inv);
+    *reinterpret_cast<uint2*>(P.o16 + (size_t)x * HD + 4 * (32 * (W > 1 ? wi : v) + lane)) = y;
+  }
+}
+
+template <int HD, int W> int launch_merge(const AttnP& P, bool bf, int slot_rows, cudaStream_t st) {
+  auto kern = bf ? paged_merge_kernel<HD, true, W> : paged_merge_kernel<HD, false, W>;
+  const long long warps = (long long)P.rows * P.nh * W;
+  return launch_pdl("paged_merge_kernel", kern, dim3((unsigned)((warps + 7) / 8)), MERGE_THREADS, 0, st, P, slot_rows);
 }
 
 int ctas_of(int hd) { return SMS * (hd == 256 ? 1 : 2); }
@@ -477,12 +469,10 @@ Work carve(void* ws, const yskn_paged_cache& c, int rows, int nh, int splits) {
   size_t at = 0;
   auto take = [&](size_t n) { const size_t x = at; at = (at + n + 255) / 256 * 256; return static_cast<uint8_t*>(ws) + x; };
   Work w;
-  w.first = reinterpret_cast<int*>(take((chunk + 1) * 4));
-  w.pm = reinterpret_cast<float*>(take(pieces * sr * 4));
-  w.pl = reinterpret_cast<float*>(take(pieces * sr * 4));
+  w.span = reinterpret_cast<int2*>(take((size_t)chunk * c.kvh * 8));
+  w.ml = reinterpret_cast<float2*>(take(pieces * sr * 8));
   w.pacc = reinterpret_cast<float*>(take(pieces * sr * c.hd * 4));
-  w.qm = reinterpret_cast<float*>(take(parts * 4));
-  w.ql = reinterpret_cast<float*>(take(parts * 4));
+  w.qml = reinterpret_cast<float2*>(take(parts * 8));
   w.qacc = reinterpret_cast<float*>(take(parts * c.hd * 4));
   w.bytes = at;
   return w;
@@ -532,13 +522,14 @@ int launch_paged_attention(const yskn_paged_cache& c, const yskn_paged_rows& r, 
     const size_t part = (size_t)first * splits * a.nh;
     AttnP P{rows_of(c, r, first), rows, g, a.nh, static_cast<const uint16_t*>(a.q) + first * a.q_stride, (long long)a.q_stride, a.qscale * LOG2E,
             static_cast<uint16_t*>(a.o16) + (size_t)first * a.nh * c.hd, splits > 0 ? a.shared : 0, a.ids ? a.ids + (size_t)first * c.kvh * a.take : nullptr, a.take,
-            w.first, w.pm, w.pl, w.pacc, w.qm + part, w.ql + part, w.qacc + part * c.hd, splits};
+            w.span, w.ml, w.pacc, w.qml + part, w.qacc + part * c.hd, splits};
     if (int rc = c.hd == 256 ? dispatch<256>(c, P, st) : dispatch<128>(c, P, st)) return rc;
-    // few rows: a block a head; many: a block a kv-head, since most of them have nothing to do
-    const int hpb = (long long)rows * a.nh <= 4 * 2 * SMS ? 1 : g;
-    auto merge = c.hd == 256 ? (c.dtype == YSKN_KV4_BF16 ? paged_merge_kernel<256, true> : paged_merge_kernel<256, false>)
-                             : (c.dtype == YSKN_KV4_BF16 ? paged_merge_kernel<128, true> : paged_merge_kernel<128, false>);
-    if (int rc = launch_pdl("paged_merge_kernel", merge, dim3((unsigned)(a.nh / hpb), (unsigned)rows), MERGE_THREADS, 0, st, P, ctas_of(c.hd), slot_rows_of(g), hpb)) return rc;
+    // few rows: their parts are many, a block adds them up together; many rows: few parts each, a warp does
+    const bool bf = c.dtype == YSKN_KV4_BF16, few = (long long)rows * a.nh <= 2 * SMS;
+    const int sr = slot_rows_of(g);
+    const int rc = c.hd == 256 ? (few ? launch_merge<256, 8>(P, bf, sr, st) : launch_merge<256, 1>(P, bf, sr, st))
+                               : (few ? launch_merge<128, 8>(P, bf, sr, st) : launch_merge<128, 1>(P, bf, sr, st));
+    if (rc) return rc;
   }
   return 0;
 }

@@ -80,10 +80,10 @@ __device__ __forceinline__ void sts128(uint32_t a, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// Workspace of one attention call.  Pieces of rows that lie on several CTAs: (m, l) and O of the heads of a kv-head; partials over the shared
-// prefix, in the layout [row][split][head]; the first tile of every row.
+// Workspace of one attention call.  Of (row, kv-head) pairs that lie on several CTAs: the first and the last, and a piece from each, (m, l) and O of the pair's heads.
+// Partials over the shared prefix, [row][split][head].
 struct Work {
-  int* first; float* pm; float* pl; float* pacc; float* qm; float* ql; float* qacc;
+  int2* span; float2* ml; float* pacc; float2* qml; float* qacc;
   size_t bytes;
 };
 

@@ -45,7 +45,7 @@ template <int HD> struct Lay {
 struct PrefixP {
   Rows R; int rows, G, tpc, nh, splits, per, tiles, shared;            // tpc rows of a CTA; per tiles of a split
   const uint16_t* q; long long qs; float cs; uint32_t flip;            // |qscale| log2 e; its sign, as sign bits of two queries
-  float* qm; float* ql; float* qacc;
+  float2* qml; float* qacc;
 };
 
 __device__ __forceinline__ bool elect_one() {
@@ -364,7 +364,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
     if (!__all_sync(0xffffffffu, ok && !*s_abort)) return;
     fence_after();
     const size_t part = ((size_t)row * P.splits + split) * P.nh + head;
-    if (valid && hf == 0) { P.qm[part] = m; P.ql[part] = l; }
+    if (valid && hf == 0) P.qml[part] = make_float2(m, l);
     constexpr int LPR = HD / 8;                                        // lanes that cover half a row
     #pragma unroll 1
     for (int c = hf * (HD / 64); c < (hf + 1) * (HD / 64); ++c) {
@@ -449,7 +449,7 @@ int launch_paged_prefix(const yskn_paged_cache& c, const yskn_paged_rows& r, con
   const int g = a.nh / c.kvh, pairs = pairs_of(r.rows, g), tpc = (r.rows + 2 * pairs - 1) / (2 * pairs), nt = tiles_of(a.shared);
   const float cs = a.qscale * LOG2E;
   PrefixP P{rows_of(c, r, 0), r.rows, g, tpc, a.nh, splits, (nt + splits - 1) / splits, nt, a.shared, static_cast<const uint16_t*>(a.q), (long long)a.q_stride,
-            cs < 0.f ? -cs : cs, cs < 0.f ? 0x80008000u : 0u, w.qm, w.ql, w.qacc};
+            cs < 0.f ? -cs : cs, cs < 0.f ? 0x80008000u : 0u, w.qml, w.qacc};
   const bool bf = c.dtype == YSKN_KV4_BF16;
   return c.hd == 256 ? (bf ? launch<256, true>(c, P, pairs, st) : launch<256, false>(c, P, pairs, st))
                      : (bf ? launch<128, true>(c, P, pairs, st) : launch<128, false>(c, P, pairs, st));

@@ -4,9 +4,8 @@
 // fp64, and a sum of HD of them in fp64 is exact or off by 2^-52 of its largest part: the choice does not depend on the order of the sum, and two builds, or a
 // plain program, agree on every block.  fp32 sums differ by 2^-24, which decides between neighbours every few thousand rows.
 //
-// Bound: the mean keys, 2 HD bytes a page and kv-head, read once per row.  B200 does fp64 at half the rate of fp32, so the G products a channel run beside the loads.
-// Two launches: scores as 64-bit keys that sort like the score (workspace); the choice, a block a (row, kv-head): digits of the keys counted from the highest
-// on until the border is found, then one walk that writes the chosen blocks in rising order.
+// Bound: the mean keys, 2 HD bytes a page and kv-head, read once per row, and fp64 products beside them, which B200 does at half the rate of fp32.
+// Two launches: scores as 64-bit keys that sort like the score (workspace); the choice, a block a (row, kv-head).
 #include "paged_common.cuh"
 
 namespace kv4 {
@@ -26,122 +25,207 @@ __device__ __forceinline__ unsigned long long key_of(double x) {
   return b < 0 ? ~(unsigned long long)b : (unsigned long long)b | 0x8000000000000000ull;
 }
 
-constexpr int SCORE_BLOCKS = 64;             // blocks of one CTA
-// A warp takes a block at a time: lane l has channels 8l .. 8l + 7 (hd 128: half a warp a block).  Queries in shared memory as fp64.
+constexpr int SCORE_WARPS = 8;
+// A warp takes a block at a time, HD / 32 channels a lane; a lane keeps its channels of up to eight heads in registers (fp64; from shared memory they would be the
+// bound: eight bytes a product).  The heads' sums are folded over the warp together: at each step a lane gives away half of what it holds.  Pages and
+// mean keys are asked for four blocks ahead of their use.
 template <int HD, bool BF>
-__global__ void __launch_bounds__(256) paged_score_kernel(const SelectP P) {
-  constexpr int LPB = HD / 8, BPW = 32 / LPB;
-  extern __shared__ double qs[];                                        // [g][HD], channel c of lane l at (c % 8) * LPB + l: lanes side by side
+__global__ void __launch_bounds__(SCORE_WARPS * 32) paged_score_kernel(const SelectP P, int per_warp) {
+  constexpr int C = HD / 32, GP = 8, AHEAD = 4;
   pdl_wait();
   pdl_launch();
   const int row = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b0 = ((int)blockIdx.x * SCORE_WARPS + warp) * per_warp;
   const Place w = place_of(P.R, row);
-  if (w.seq < 0) return;
-  const int n = w.vis > 0 ? (w.vis - 1) >> P.R.lp : 0;                  // candidates: blocks in front of the last
-  const int b0 = (int)blockIdx.x * SCORE_BLOCKS;
-  if (b0 >= n) return;
-  for (int i = threadIdx.x; i < P.g * (HD / 2); i += 256) {
-    const int gi = i / (HD / 2), c = 2 * (i % (HD / 2));
-    const float2 f = unpack16<BF>(*reinterpret_cast<const uint32_t*>(P.q + row * P.qs + (size_t)(h * P.g + gi) * HD + c));
-    double* d = qs + gi * HD + c / 8;
-    d[(c & 7) * LPB] = f.x; d[((c & 7) + 1) * LPB] = f.y;
-  }
-  __syncthreads();
-  const int l = lane % LPB;
-  #pragma unroll 1
-  for (int i = warp * BPW + lane / LPB; i < SCORE_BLOCKS; i += 8 * BPW) {
-    const int b = b0 + i;
-    const int page = b < n ? page_of(P.R, w.seq, b) : -1;
-    double x[8];
-    uint4 u = make_uint4(0u, 0u, 0u, 0u);
-    if (page >= 0) u = *reinterpret_cast<const uint4*>(P.kmean + ((size_t)page * P.R.kvh + h) * HD + 8 * l);
-    const uint32_t u4[4] = {u.x, u.y, u.z, u.w};
+  const int n = w.seq >= 0 && w.vis > 0 ? (w.vis - 1) >> P.R.lp : 0;    // candidates: blocks in front of the last
+  const int b1 = min(n, b0 + per_warp);
+  if (b0 >= b1) return;
+  unsigned long long* keys = P.keys + ((size_t)row * P.R.kvh + h) * P.R.blocks;
+  for (int g0 = 0; g0 < P.g; g0 += GP) {                                // more than eight heads: in two walks
+    const int gn = min(GP, P.g - g0);
+    double q[GP][C];
     #pragma unroll
-    for (int e = 0; e < 4; ++e) { const float2 f = unpack16<BF>(u4[e]); x[2 * e] = f.x; x[2 * e + 1] = f.y; }
-    double best = 0.0;
-    bool any = false;
-    for (int gi = 0; gi < P.g; ++gi) {
-      const double* q = qs + gi * HD + l;
-      double a = 0.0, b2 = 0.0;
+    for (int i = 0; i < GP; ++i) {
+      const uint16_t* src = P.q + row * P.qs + (size_t)(h * P.g + g0 + min(i, gn - 1)) * HD + C * lane;
       #pragma unroll
-      for (int e = 0; e < 8; e += 2) { a = fma(q[e * LPB], x[e], a); b2 = fma(q[(e + 1) * LPB], x[e + 1], b2); }
-      a += b2;
-      #pragma unroll
-      for (int d = LPB / 2; d > 0; d >>= 1) a += __shfl_xor_sync(0xffffffffu, a, d);
-      if (a == a) { best = any ? fmax(best, a) : a; any = true; }
+      for (int e = 0; e < C / 2; ++e) { const float2 f = unpack16<BF>(reinterpret_cast<const uint32_t*>(src)[e]); q[i][2 * e] = f.x; q[i][2 * e + 1] = f.y; }
     }
-    if (l == 0 && b < n) P.keys[((size_t)row * P.R.kvh + h) * P.R.blocks + b] = page < 0 ? 0ull : any ? key_of(best) : 1ull;
+    for (int bb = b0; bb < b1; bb += 32) {
+      const int mine = bb + lane < b1 ? page_of(P.R, w.seq, bb + lane) : -1;
+      const int m = min(32, b1 - bb);
+      uint32_t u[AHEAD][C / 2];
+      auto ask = [&](int i, uint32_t (&x)[C / 2]) {
+        const int page = __shfl_sync(0xffffffffu, mine, i & 31);
+        const uint16_t* src = P.kmean + ((size_t)max(page, 0) * P.R.kvh + h) * HD + C * lane;          // no page: any, its key is overwritten
+        if constexpr (C == 8) { const uint4 v = *reinterpret_cast<const uint4*>(src); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
+        else { const uint2 v = *reinterpret_cast<const uint2*>(src); x[0] = v.x; x[1] = v.y; }
+      };
+      #pragma unroll
+      for (int i = 0; i < AHEAD; ++i) ask(i, u[i]);
+      for (int i0 = 0; i0 < m; i0 += AHEAD) {
+        #pragma unroll
+        for (int a = 0; a < AHEAD; ++a) {
+          double x[C], s[GP];
+          #pragma unroll
+          for (int e = 0; e < C / 2; ++e) { const float2 f = unpack16<BF>(u[a][e]); x[2 * e] = f.x; x[2 * e + 1] = f.y; }
+          ask(i0 + a + AHEAD, u[a]);
+          #pragma unroll
+          for (int i = 0; i < GP; ++i) {
+            s[i] = 0.0;
+            if (i < gn) {
+              #pragma unroll
+              for (int e = 0; e < C; ++e) s[i] = fma(q[i][e], x[e], s[i]);
+            }
+          }
+          // 8 -> 4 -> 2 -> 1 sums a lane; lane bits 4, 3, 2 are then the head, and two more steps finish its sum
+          #pragma unroll
+          for (int d = 16, c = GP / 2; c >= 1; d >>= 1, c >>= 1) {
+            const bool up = (lane & d) != 0;
+            #pragma unroll
+            for (int i = 0; i < GP / 2; ++i)
+              if (i < c) { const double give = up ? s[i] : s[i + c], keep = up ? s[i + c] : s[i]; s[i] = keep + __shfl_xor_sync(0xffffffffu, give, d); }
+          }
+          double t = s[0];
+          t += __shfl_xor_sync(0xffffffffu, t, 2);
+          t += __shfl_xor_sync(0xffffffffu, t, 1);
+          unsigned long long key = (lane >> 2) < gn ? key_of(t) : 0ull;
+          #pragma unroll
+          for (int d = 16; d >= 4; d >>= 1) { const unsigned long long o = __shfl_xor_sync(0xffffffffu, key, d); key = o > key ? o : key; }
+          const int i = i0 + a, page = __shfl_sync(0xffffffffu, mine, i & 31);
+          if (lane == 0 && i < m) {
+            if (g0 > 0) { const unsigned long long o = keys[bb + i]; key = o > key ? o : key; }
+            keys[bb + i] = page < 0 ? 0ull : key;
+          }
+        }
+      }
+    }
   }
 }
 
-// The choice.  Keys of equal height are taken from the lowest block on.  Digits of 8 bits from the top: how many keys share the digits so far, until what is left to
-// take is all of them or the digits are used up.
-__global__ void __launch_bounds__(256) paged_choose_kernel(const SelectP P) {
-  __shared__ int hist[256], warps[8], s_digit, s_left, s_all;
+// The choice.  The highest keys' range is cut into 2,048 bins at a time, from the highest bit in which the keys differ on: the bin that holds the last place, then, where it holds
+// few keys, the place in it by counting for each how many come before it; otherwise its bins in turn.  Keys of equal height are taken from the lowest block on.
+// Then one walk writes the chosen blocks in rising order.
+constexpr int CT = 512, BINS = 2048, LIST = 256;
+__global__ void __launch_bounds__(CT) paged_choose_kernel(const SelectP P) {
+  __shared__ unsigned long long s_hi[CT / 32], s_lo[CT / 32], list[LIST], s_cut;
+  __shared__ int hist[BINS], warps[CT / 32], s_bin, s_left, s_count, s_n;
   pdl_wait();
   pdl_launch();
-  const int row = blockIdx.y, h = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Place w = place_of(P.R, row);
   if (w.seq < 0) return;
   const size_t pair = (size_t)row * P.R.kvh + h;
   const unsigned long long* keys = P.keys + pair * P.R.blocks;
   int* ids = P.ids + pair * P.take;
   const int last = w.vis > 0 ? (w.vis - 1) >> P.R.lp : -1, n = last > 0 ? last : 0;
-  // ---- the border: keys above `low` are taken, and of those equal to it the first `left`
-  unsigned long long prefix = 0, mask = 0;
+
+  // ---- highest and lowest candidate, and how many there are
+  unsigned long long hi = 0, lo = ~0ull;
+  int count = 0;
+  #pragma unroll 4
+  for (int i = tid; i < n; i += CT) { const unsigned long long k = keys[i]; if (k) { hi = k > hi ? k : hi; lo = k < lo ? k : lo; ++count; } }
+  #pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    const unsigned long long a = __shfl_xor_sync(0xffffffffu, hi, d), b = __shfl_xor_sync(0xffffffffu, lo, d);
+    hi = a > hi ? a : hi; lo = b < lo ? b : lo; count += __shfl_xor_sync(0xffffffffu, count, d);
+  }
+  if (lane == 0) { s_hi[warp] = hi; s_lo[warp] = lo; warps[warp] = count; }
+  __syncthreads();
+  count = 0;
+  #pragma unroll
+  for (int i = 0; i < CT / 32; ++i) { hi = s_hi[i] > hi ? s_hi[i] : hi; lo = s_lo[i] < lo ? s_lo[i] : lo; count += warps[i]; }
+  __syncthreads();
+
+  // ---- the border: keys above `cut` are taken, and of those equal to it the first `left`
+  unsigned long long cut = 0;
   int left = P.take - 1;
-  bool all = n <= left;                                                 // every candidate
-  for (int shift = 56; shift >= 0 && !all; shift -= 8) {
-    hist[threadIdx.x] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += 256) {
-      const unsigned long long k = keys[i];
-      if ((k & mask) == prefix && k != 0) atomicAdd(&hist[(int)(k >> shift) & 255], 1);
+  if (count > left && hi == lo) cut = hi;                               // all alike
+  else if (count > left) {
+    int top = 64 - __clzll((long long)(hi ^ lo));                       // the keys that are still looked at have `fixed` from bit `top` on
+    unsigned long long fixed = top < 64 ? hi >> top : 0ull;
+    auto looked = [&](unsigned long long k) { return k && (top < 64 ? k >> top : 0ull) == fixed; };
+    for (;;) {
+      const int shift = max(0, top - 11);
+      for (int i = tid; i < BINS; i += CT) hist[i] = 0;
+      if (tid == 0) s_n = 0;
+      __syncthreads();
+      for (int i = tid; i < n; i += CT) {
+        const unsigned long long k = keys[i];
+        if (looked(k)) atomicAdd(&hist[(int)(k >> shift) & ((1 << (top - shift)) - 1)], 1);
+      }
+      __syncthreads();
+      // thread t has bins BINS - 1 - 4t and the three below: how many keys lie above them
+      int c4[4], mine = 0;
+      #pragma unroll
+      for (int e = 0; e < 4; ++e) { c4[e] = hist[BINS - 1 - 4 * tid - e]; mine += c4[e]; }
+      int upto = mine;
+      #pragma unroll
+      for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
+      if (lane == 31) warps[warp] = upto;
+      __syncthreads();
+      for (int i = 0; i < warp; ++i) upto += warps[i];
+      int above = upto - mine;
+      #pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (above < left && above + c4[e] >= left) { s_bin = BINS - 1 - 4 * tid - e; s_left = left - above; s_count = c4[e]; }
+        above += c4[e];
+      }
+      __syncthreads();
+      left = s_left;
+      fixed = fixed << (top - shift) | (unsigned long long)s_bin;
+      top = shift;
+      const int in_bin = s_count;
+      if (shift == 0) { cut = fixed; break; }                           // equal keys
+      if (in_bin <= LIST) {
+        for (int i = tid; i < n; i += CT) { const unsigned long long k = keys[i]; if (looked(k)) list[atomicAdd(&s_n, 1)] = k; }
+        __syncthreads();
+        if (tid < in_bin) {                                             // the `left`-th of the list from the top; of equal keys any thread may say it
+          const unsigned long long k = list[tid];
+          int more = 0, same = 0;
+          for (int i = 0; i < in_bin; ++i) { more += list[i] > k; same += list[i] == k; }
+          if (more < left && more + same >= left) { s_cut = k; s_left = left - more; }
+        }
+        __syncthreads();
+        cut = s_cut; left = s_left;
+        break;
+      }
+      __syncthreads();
     }
-    __syncthreads();
-    // thread t stands for digit 255 - t: keys of higher digits in front
-    const int mine = hist[255 - threadIdx.x];
+  }
+  __syncthreads();
+  // ---- one walk in rising order, four blocks a thread
+  int at = 0, equal = 0;                                                // taken so far; keys equal to the border so far
+  for (int i0 = 0; i0 < n; i0 += 4 * CT) {
+    unsigned long long k4[4];
+    int mine = 0;                                                       // keys above the border, and equal ones << 16
+    #pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = i0 + 4 * tid + e;
+      k4[e] = i < n ? keys[i] : 0ull;
+      mine += k4[e] > cut ? 1 : k4[e] && k4[e] == cut ? 1 << 16 : 0;
+    }
     int upto = mine;
     #pragma unroll
     for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
     if (lane == 31) warps[warp] = upto;
-    if (threadIdx.x == 0) s_all = 0;
     __syncthreads();
-    for (int i = 0; i < warp; ++i) upto += warps[i];
-    if (upto - mine < left && upto >= left) { s_digit = 255 - threadIdx.x; s_left = left - (upto - mine); s_all = upto == left ? 1 : 0; }
-    if (threadIdx.x == 255 && upto < left) s_all = 2;                   // fewer candidates than places: all of them
-    __syncthreads();
-    if (s_all == 2) { all = true; break; }
-    prefix |= (unsigned long long)s_digit << shift; mask |= 255ull << shift;
-    left = s_left;
-    const bool done = s_all == 1;                                       // all keys with these digits are taken
-    __syncthreads();
-    if (done) break;
-  }
-  // ---- one walk in rising order
-  int at = 0;                                                           // taken so far; `equal` of them with the border's digits
-  int equal = 0;
-  for (int i0 = 0; i0 < n; i0 += 256) {
-    const int i = i0 + (int)threadIdx.x;
-    const unsigned long long k = i < n ? keys[i] : 0ull;
-    const bool eq = !all && k != 0 && (k & mask) == prefix;
-    const bool above = k != 0 && (all || (k & mask) > prefix);
-    const unsigned be = __ballot_sync(0xffffffffu, eq), ba = __ballot_sync(0xffffffffu, above), under = (1u << lane) - 1u;
-    if (lane == 0) warps[warp] = __popc(be) << 16 | __popc(ba);
-    __syncthreads();
-    int e = equal, a = 0, te = 0, ta = 0;
+    int before = upto - mine, all = 0;
     #pragma unroll
-    for (int x = 0; x < 8; ++x) { const int v = warps[x]; if (x < warp) { e += v >> 16; a += v & 0xffff; } te += v >> 16; ta += v & 0xffff; }
-    e += __popc(be & under); a += __popc(ba & under);
-    const int eq_before = min(e, left) - min(equal, left);              // equal keys taken among this walk's lower ones
-    if ((eq && e < left) || above) ids[at + a + eq_before] = i;
-    at += ta + min(equal + te, left) - min(equal, left);
-    equal += te;
+    for (int i = 0; i < CT / 32; ++i) { const int v = warps[i]; if (i < warp) before += v; all += v; }
+    int a = before & 0xffff, e0 = equal + (before >> 16);
+    #pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool eq = k4[e] && k4[e] == cut, take = k4[e] > cut || (eq && e0 < left);
+      if (take) ids[at + a + min(e0, left) - min(equal, left)] = i0 + 4 * tid + e;
+      a += k4[e] > cut; e0 += eq;
+    }
+    at += (all & 0xffff) + min(equal + (all >> 16), left) - min(equal, left);
+    equal += all >> 16;
     __syncthreads();
   }
-  if (threadIdx.x == 0 && last >= 0) ids[at] = last;
+  if (tid == 0 && last >= 0) ids[at] = last;
   if (last >= 0) ++at;
-  for (int i = at + (int)threadIdx.x; i < P.take; i += 256) ids[i] = -1;
+  for (int i = at + tid; i < P.take; i += CT) ids[i] = -1;
 }
 
 }  // namespace
@@ -157,10 +241,15 @@ int launch_paged_select(const yskn_paged_cache& c, const yskn_paged_rows& r, con
             static_cast<unsigned long long*>(a.workspace), a.take, a.ids};
   auto score = c.hd == 256 ? (bf ? paged_score_kernel<256, true> : paged_score_kernel<256, false>)
                            : (bf ? paged_score_kernel<128, true> : paged_score_kernel<128, false>);
-  if (r.blocks > 1)
-    if (int rc = launch_pdl("paged_score_kernel", score, dim3((unsigned)((r.blocks - 1 + SCORE_BLOCKS - 1) / SCORE_BLOCKS), (unsigned)c.kvh, (unsigned)r.rows), 256,
-                            (size_t)g * c.hd * 8, st, P)) return rc;
-  return launch_pdl("paged_choose_kernel", paged_choose_kernel, dim3((unsigned)c.kvh, (unsigned)r.rows), 256, 0, st, P);
+  if (r.blocks > 1) {
+    // blocks of a warp: as many as leave two CTAs an SM, since a CTA's start (its queries as fp64) costs what eight blocks do
+    int per = 4;
+    while (per < 64 && (long long)r.rows * c.kvh * ((r.blocks - 1) / (SCORE_WARPS * 2 * per)) >= 2 * SMS) per *= 2;
+    const int cta = SCORE_WARPS * per;
+    if (int rc = launch_pdl("paged_score_kernel", score, dim3((unsigned)((r.blocks - 1 + cta - 1) / cta), (unsigned)c.kvh, (unsigned)r.rows), SCORE_WARPS * 32, 0, st, P, per))
+      return rc;
+  }
+  return launch_pdl("paged_choose_kernel", paged_choose_kernel, dim3((unsigned)c.kvh, (unsigned)r.rows), CT, 0, st, P);
 }
 
 }  // namespace kv4
