@@ -45,7 +45,7 @@ struct AttnP {
 template <int HD, int NT> struct Lay {
   static constexpr int HALF = TILE * HD * 2, QP = HD * 2 + 16, PP = TILE * 2 + 16;   // bytes: a half stage; a row of Q; a row of P (paddings: eight rows on different banks)
   static constexpr int OFF_Q = NSLOT * HALF, OFF_P = OFF_Q + 2 * NT * 8 * QP, OFF_MAX = OFF_P + 2 * NT * 8 * PP, OFF_L = OFF_MAX + 2 * CW * NT * 8 * 4;
-  static constexpr int OFF_BASE = OFF_L + CW * NT * 8 * 4, OFF_BAR = OFF_BASE + 3 * 4 * 4, OFF_SUM = OFF_BAR + 16 * 8 + 8, OFF_PLACE = OFF_SUM + 32, OFF_FIRST = OFF_PLACE + ROWS * 8;
+  static constexpr int OFF_BASE = OFF_L + CW * NT * 8 * 4, OFF_BAR = OFF_BASE + 3 * 4 * 4, OFF_PLACE = OFF_BAR + 16 * 8 + 8, OFF_FIRST = OFF_PLACE + ROWS * 8;
   static constexpr int TOTAL = OFF_FIRST + (ROWS + 1) * 4;
   static constexpr int CTAS = HD == 256 ? 1 : 2;
   static_assert(HALF % 1024 == 0 && OFF_BASE % 16 == 0 && OFF_BAR % 8 == 0 && CTAS * (TOTAL + 1024) <= 228 * 1024, "shared memory");
@@ -86,43 +86,36 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
   const uint32_t b_full = sb + L::OFF_BAR, b_empty = b_full + 8 * NSLOT, b_qfull = b_empty + 8 * NSLOT, b_qempty = b_qfull + 16;
   volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::OFF_BAR + 16 * 8);
   int* first = reinterpret_cast<int*>(smem + L::OFF_FIRST);
-  int* sums = reinterpret_cast<int*>(smem + L::OFF_SUM);
   Place* places = reinterpret_cast<Place*>(smem + L::OFF_PLACE);
   if (threadIdx.x == 0) {
     for (int i = 0; i < NSLOT; ++i) { bar_init(b_full + 8 * i, 1); bar_init(b_empty + 8 * i, CW); }
     for (int i = 0; i < 2; ++i) { bar_init(b_qfull + 8 * i, 1); bar_init(b_qempty + 8 * i, CW); }
     *s_abort = sb & 1023u ? 1 : 0;           // the swizzled tiles need a base of 1 KB
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mapK) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mapV) : "memory");
   }
+  __syncthreads();
   pdl_wait();
   pdl_launch();
 
-  // ---- the line: first[r] = tiles of one kv-head ahead of row r
+  // ---- the line: first[r] = tiles of one kv-head ahead of row r.  Every warp finds it for itself (all write the same): no barrier between the positions and the first copy
   {
-    constexpr int PER = ROWS / 128;
-    int n[PER], mine = 0, below = 0;
-    if (warp < CW) {
-      #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int r = (int)threadIdx.x * PER + i;
-        n[i] = 0;
-        if (r < P.rows) { const Place w = place_of(P.R, r); places[r] = w; n[i] = tiles_of(P, w); }
-        mine += n[i];
+    int below = 0;
+    for (int r0 = 0; r0 < ROWS; r0 += 32) {
+      const int r = r0 + lane;
+      int mine = 0;
+      if (r < P.rows) { const Place w = place_of(P.R, r); places[r] = w; mine = tiles_of(P, w); }
+      int upto = mine;
+      if (r0 < P.rows) {
+        #pragma unroll
+        for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
       }
-      below = mine;
-      #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, below, d); if (lane >= d) below += o; }
-      if (lane == 31) sums[warp] = below;
-      below -= mine;
+      first[r] = below + upto - mine;
+      below += __shfl_sync(0xffffffffu, upto, 31);
     }
-    __syncthreads();
-    if (warp < CW) {
-      for (int i = 0; i < warp; ++i) below += sums[i];
-      #pragma unroll
-      for (int i = 0; i < PER; ++i) { first[threadIdx.x * PER + i] = below; below += n[i]; }
-      if (threadIdx.x == 127) first[ROWS] = below;
-    }
-    __syncthreads();
+    if (lane == 0) first[ROWS] = below;
+    __syncwarp();
   }
   const int kvh = P.R.kvh, total = first[ROWS] * kvh, grid = min((int)gridDim.x, total), cta = (int)blockIdx.x;       // every CTA below `grid` has a tile at least
   if (cta >= grid) return;
@@ -168,10 +161,12 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     int k = 0, pair = -1, issued = 0, queries = 0;                     // tiles so far; the pair they belong to; half stages and queries asked for
     bool ok = *s_abort == 0;
     const int tpb = 32 / npt, jl = lane & (npt - 1), tl = lane / npt;  // tiles of a batch; this lane's box and tile in it
-    Box now = box_of(u0 + tl, jl), next = box_of(u0 + tpb + tl, jl);
+    Box now = box_of(u0 + tl, jl), next = now;
     for (int u = u0; u < u1 && ok; ++u, ++k) {
       int i = u - u0;
-      if (i > 0 && i % tpb == 0) { now = next; next = box_of(u + tpb + tl, jl); }
+      if (i > 0 && i % tpb == 0) now = next;
+      const bool look = i % tpb == min(3, tpb - 1);                    // for the next batch, once the ring is full
+      const int behind = u - i % tpb + tpb + tl;
       i = (i % tpb) * npt + jl;
       const int at = __shfl_sync(0xffffffffu, now.at, i), base = __shfl_sync(0xffffffffu, now.base, i), pr = __shfl_sync(0xffffffffu, now.pair, i);
       if (pr != pair) {                                                // queries of the next pair
@@ -198,6 +193,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
         ++issued;
         if (lane < npt) tma_3d(sb + slot * L::HALF + lane * (chunk * HD * 2), v ? &mapV : &mapK, 0, at, 0, b_full + 8 * slot);
       }
+      if (look) next = box_of(behind, jl);
     }
     if (!ok) {                                                         // give up; the copies under way land before the block ends
       if (lane == 0) { atomicExch(&g_attn_status, 7); *s_abort = 1; }
@@ -409,8 +405,24 @@ __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnP 
   const size_t piece0 = ((size_t)span.x + pair) * slot_rows + hh;      // piece c of the pair: + c * slot_rows
   auto ml_at = [&](int i) { return i < np ? qml[(size_t)i * P.nh] : P.ml[piece0 + (size_t)(i - np) * slot_rows]; };
   auto o_at = [&](int i) { return i < np ? qacc + (size_t)i * P.nh * HD : P.pacc + (piece0 + (size_t)(i - np) * slot_rows) * HD; };
-  float top = -INFINITY;
-  for (int i = lane; i < n; i += 32) { const float2 f = ml_at(i); if (f.y != 0.f) top = fmaxf(top, f.x); }
+  constexpr int U = W > 1 ? 8 : 4, PC = U * W;           // parts that a warp asks for together; parts of all W warps
+  auto ml_or = [&](int i) { return i < n ? ml_at(i) : make_float2(-INFINITY, 0.f); };
+  float4 o[U][V];
+  auto ask = [&](int c) {                    // O of this warp's parts c + wi + W u: beside the maxima and sums, not behind them
+    #pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = c + wi + W * u;
+      if (i < n) {
+        const float4* src = reinterpret_cast<const float4*>(o_at(i)) + lane;
+        #pragma unroll
+        for (int v = 0; v < V; ++v) o[u][v] = src[32 * v];
+      }
+    }
+  };
+  float2 f0 = ml_or(lane), f1 = ml_or(32 + lane);
+  ask(0);
+  float top = fmaxf(f0.y != 0.f ? f0.x : -INFINITY, f1.y != 0.f ? f1.x : -INFINITY);
+  for (int i = 64 + lane; i < n; i += 32) { const float2 f = ml_at(i); if (f.y != 0.f) top = fmaxf(top, f.x); }
   #pragma unroll
   for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   if (top == -INFINITY) top = 0.f;
@@ -418,18 +430,17 @@ __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnP 
   float4 acc[V];
   #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    float wt = 0.f;
-    if (i0 + lane < n) { const float2 f = ml_at(i0 + lane); if (f.y != 0.f) { wt = ex2(f.x - top); sum += f.y * wt; } }
-    const int m = min(32, n - i0);
-    #pragma unroll 4
-    for (int k = wi; k < m; k += W) {
-      const float wk = __shfl_sync(0xffffffffu, wt, k);
-      const float4* src = reinterpret_cast<const float4*>(o_at(i0 + k)) + lane;
-      #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float4 f = src[32 * v];
-        if (wk != 0.f) { acc[v].x += wk * f.x; acc[v].y += wk * f.y; acc[v].z += wk * f.z; acc[v].w += wk * f.w; }      // a part without weight may hold anything
+  for (int c = 0; c < n; c += PC) {
+    if (c > 0) { f0 = ml_or(c + lane); f1 = PC > 32 ? ml_or(c + 32 + lane) : f1; ask(c); }
+    const float w0 = lane < PC && f0.y != 0.f ? ex2(f0.x - top) : 0.f, w1 = PC > 32 && f1.y != 0.f ? ex2(f1.x - top) : 0.f;
+    if (lane < PC && f0.y != 0.f) sum += f0.y * w0;
+    if (PC > 32 && f1.y != 0.f) sum += f1.y * w1;
+    #pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float wk = __shfl_sync(0xffffffffu, W * u < 32 ? w0 : w1, (wi + W * u) & 31);
+      if (wk != 0.f) {                       // a part without weight may hold anything
+        #pragma unroll
+        for (int v = 0; v < V; ++v) { acc[v].x += wk * o[u][v].x; acc[v].y += wk * o[u][v].y; acc[v].z += wk * o[u][v].z; acc[v].w += wk * o[u][v].w; }
       }
     }
   }

@@ -1,255 +1,391 @@
 // Choice of the blocks that a row attends to (sm_100a): a score for every complete page, then the highest ones.
 //
-// Mathematics: score(b) = max over the heads h of a kv-head's group of sum_c q_h[c] mean_b[c].  Products of two 16-bit values are exact in fp32, and all the more so in
-// fp64, and a sum of HD of them in fp64 is exact or off by 2^-52 of its largest part: the choice does not depend on the order of the sum, and two builds, or a
-// plain program, agree on every block.  fp32 sums differ by 2^-24, which decides between neighbours every few thousand rows.
+// Mathematics: score(b) = max over the heads h of a kv-head's group of sum_c q_h[c] mean_b[c].  The choice is the one that fp64 sums make: products of two 16-bit values
+// are exact there, and a sum of HD of them is exact or off by 2^-52 of its largest part, so that the choice depends on no order of a sum.  fp64 sums of everything
+// were fp64-bound, though (16 rows of 7 heads over 65,536 tokens: 28 us for 15 MB of mean keys).  So:
+//   1. scores on the tensor cores: exact products, fp32 sums, off by at most e = HD 2^-21 * max over blocks and heads of sum_c |q_h[c] mean_b[c]|, which a second
+//      product yields (HD / 16 instructions of 16 products and a sum each, truncated at 2^-23 of the largest: (17/16) HD 2^-23 of that sum; a factor of about four is margin);
+//   2. with t the (take - 1)-th highest of them: what is above t + 2e is among the chosen, what is below t - 2e is not, for at least take - 1 exact scores are
+//      t - e or more, and at most take - 2 are above t + e; what lies between, a block or two, is scored in fp64.
+// Where a score or e is not finite everything is scored in fp64.
 //
-// Bound: the mean keys, 2 HD bytes a page and kv-head, read once per row, and fp64 products beside them, which B200 does at half the rate of fp32.
-// Two launches: scores as 64-bit keys that sort like the score (workspace); the choice, a block a (row, kv-head).
+// Bound: the mean keys, 2 HD bytes a page and kv-head, read once per row.
 #include "paged_common.cuh"
 
 namespace kv4 {
 namespace paged {
 namespace {
 
+typedef unsigned long long u64;
+
 struct SelectP {
   Rows R; int rows, g, nh;
   const uint16_t* q; long long qs; const uint16_t* kmean;
-  unsigned long long* keys; int take; int* ids;
+  float2* approx; u64* exact;                // [row][kv-head][block]: score and sum of |q mean| (negative: no page); fp64 score as a sortable key, where it is needed
+  int take; int* ids;
 };
 
-// A number's bits as an unsigned integer of the same order; 0 for what is no candidate, 1 for a score that is not a number.
-__device__ __forceinline__ unsigned long long key_of(double x) {
-  if (x != x) return 1ull;
-  const long long b = __double_as_longlong(x + 0.0);                    // -0 counts as 0
-  return b < 0 ? ~(unsigned long long)b : (unsigned long long)b | 0x8000000000000000ull;
+template <bool BF> __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (BF) asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+              : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+           : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-constexpr int SCORE_WARPS = 8;
-// A warp takes a block at a time, HD / 32 channels a lane; a lane keeps its channels of up to eight heads in registers (fp64; from shared memory they would be the
-// bound: eight bytes a product).  The heads' sums are folded over the warp together: at each step a lane gives away half of what it holds.  Pages and
-// mean keys are asked for four blocks ahead of their use.
-template <int HD, bool BF>
-__global__ void __launch_bounds__(SCORE_WARPS * 32) paged_score_kernel(const SelectP P, int per_warp) {
-  constexpr int C = HD / 32, GP = 8, AHEAD = 4;
+// A warp takes sixteen blocks.  The contraction's order is free, so lane (g, j) reads channels 64 s + 16 j .. + 15 of its two blocks and of its head as they lie, 32 bytes
+// at a time, and takes two pairs of them for each of four instructions.
+constexpr int SCORE_WARPS = 4;
+template <int HD, bool BF, int NT>
+__global__ void __launch_bounds__(SCORE_WARPS * 32) paged_score_kernel(const SelectP P) {
+  constexpr int S = HD / 64;
   pdl_wait();
   pdl_launch();
-  const int row = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int b0 = ((int)blockIdx.x * SCORE_WARPS + warp) * per_warp;
-  const Place w = place_of(P.R, row);
-  const int n = w.seq >= 0 && w.vis > 0 ? (w.vis - 1) >> P.R.lp : 0;    // candidates: blocks in front of the last
-  const int b1 = min(n, b0 + per_warp);
-  if (b0 >= b1) return;
-  unsigned long long* keys = P.keys + ((size_t)row * P.R.kvh + h) * P.R.blocks;
-  for (int g0 = 0; g0 < P.g; g0 += GP) {                                // more than eight heads: in two walks
-    const int gn = min(GP, P.g - g0);
-    double q[GP][C];
+  const int row = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31, g8 = lane >> 2, j = lane & 3;
+  const int b0 = ((int)blockIdx.x * SCORE_WARPS + (int)(threadIdx.x >> 5)) * 16;
+  uint4 q[NT][S][2];
+  #pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const uint4* src = reinterpret_cast<const uint4*>(P.q + row * P.qs + (size_t)(h * P.g + min(8 * n + g8, P.g - 1)) * HD + 16 * j);
     #pragma unroll
-    for (int i = 0; i < GP; ++i) {
-      const uint16_t* src = P.q + row * P.qs + (size_t)(h * P.g + g0 + min(i, gn - 1)) * HD + C * lane;
+    for (int s = 0; s < S; ++s) { q[n][s][0] = src[8 * s]; q[n][s][1] = src[8 * s + 1]; }
+  }
+  const Place w = place_of(P.R, row);
+  const int n_cand = w.seq >= 0 && w.vis > 0 ? (w.vis - 1) >> P.R.lp : 0;          // candidates: blocks in front of the last
+  if (b0 >= n_cand) return;
+  const int mine = b0 + (lane & 15) < n_cand ? page_of(P.R, w.seq, b0 + (lane & 15)) : -1;
+  uint4 a[2][S][2];
+  #pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int page = max(0, __shfl_sync(0xffffffffu, mine, g8 + 8 * r));           // no page: any, the result is not used
+    const uint4* src = reinterpret_cast<const uint4*>(P.kmean + ((size_t)page * P.R.kvh + h) * HD + 16 * j);
+    #pragma unroll
+    for (int s = 0; s < S; ++s) { a[r][s][0] = src[8 * s]; a[r][s][1] = src[8 * s + 1]; }
+  }
+  float c[NT][4], m[NT][4];                  // scores; sums of the products' magnitudes
+  #pragma unroll
+  for (int n = 0; n < NT; ++n)
+    #pragma unroll
+    for (int e = 0; e < 4; ++e) c[n][e] = m[n][e] = 0.f;
+  constexpr uint32_t ABS = 0x7fff7fffu;
+  #pragma unroll
+  for (int s = 0; s < S; ++s)
+    #pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t x[4] = {a[0][s][i].x, a[0][s][i].y, a[0][s][i].z, a[0][s][i].w}, y[4] = {a[1][s][i].x, a[1][s][i].y, a[1][s][i].z, a[1][s][i].w};
       #pragma unroll
-      for (int e = 0; e < C / 2; ++e) { const float2 f = unpack16<BF>(reinterpret_cast<const uint32_t*>(src)[e]); q[i][2 * e] = f.x; q[i][2 * e + 1] = f.y; }
-    }
-    for (int bb = b0; bb < b1; bb += 32) {
-      const int mine = bb + lane < b1 ? page_of(P.R, w.seq, bb + lane) : -1;
-      const int m = min(32, b1 - bb);
-      uint32_t u[AHEAD][C / 2];
-      auto ask = [&](int i, uint32_t (&x)[C / 2]) {
-        const int page = __shfl_sync(0xffffffffu, mine, i & 31);
-        const uint16_t* src = P.kmean + ((size_t)max(page, 0) * P.R.kvh + h) * HD + C * lane;          // no page: any, its key is overwritten
-        if constexpr (C == 8) { const uint4 v = *reinterpret_cast<const uint4*>(src); x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w; }
-        else { const uint2 v = *reinterpret_cast<const uint2*>(src); x[0] = v.x; x[1] = v.y; }
-      };
-      #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) ask(i, u[i]);
-      for (int i0 = 0; i0 < m; i0 += AHEAD) {
-        #pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-          double x[C], s[GP];
-          #pragma unroll
-          for (int e = 0; e < C / 2; ++e) { const float2 f = unpack16<BF>(u[a][e]); x[2 * e] = f.x; x[2 * e + 1] = f.y; }
-          ask(i0 + a + AHEAD, u[a]);
-          #pragma unroll
-          for (int i = 0; i < GP; ++i) {
-            s[i] = 0.0;
-            if (i < gn) {
-              #pragma unroll
-              for (int e = 0; e < C; ++e) s[i] = fma(q[i][e], x[e], s[i]);
-            }
-          }
-          // 8 -> 4 -> 2 -> 1 sums a lane; lane bits 4, 3, 2 are then the head, and two more steps finish its sum
-          #pragma unroll
-          for (int d = 16, c = GP / 2; c >= 1; d >>= 1, c >>= 1) {
-            const bool up = (lane & d) != 0;
-            #pragma unroll
-            for (int i = 0; i < GP / 2; ++i)
-              if (i < c) { const double give = up ? s[i] : s[i + c], keep = up ? s[i + c] : s[i]; s[i] = keep + __shfl_xor_sync(0xffffffffu, give, d); }
-          }
-          double t = s[0];
-          t += __shfl_xor_sync(0xffffffffu, t, 2);
-          t += __shfl_xor_sync(0xffffffffu, t, 1);
-          unsigned long long key = (lane >> 2) < gn ? key_of(t) : 0ull;
-          #pragma unroll
-          for (int d = 16; d >= 4; d >>= 1) { const unsigned long long o = __shfl_xor_sync(0xffffffffu, key, d); key = o > key ? o : key; }
-          const int i = i0 + a, page = __shfl_sync(0xffffffffu, mine, i & 31);
-          if (lane == 0 && i < m) {
-            if (g0 > 0) { const unsigned long long o = keys[bb + i]; key = o > key ? o : key; }
-            keys[bb + i] = page < 0 ? 0ull : key;
-          }
-        }
+      for (int n = 0; n < NT; ++n) {
+        const uint4 b = q[n][s][i];
+        mma<BF>(c[n], x[0], y[0], x[1], y[1], b.x, b.y);
+        mma<BF>(m[n], x[0] & ABS, y[0] & ABS, x[1] & ABS, y[1] & ABS, b.x & ABS, b.y & ABS);
+        mma<BF>(c[n], x[2], y[2], x[3], y[3], b.z, b.w);
+        mma<BF>(m[n], x[2] & ABS, y[2] & ABS, x[3] & ABS, y[3] & ABS, b.z & ABS, b.w & ABS);
       }
     }
+  #pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    float best = -INFINITY, mag = 0.f;       // mag: infinity where a head's sum is no number, or beyond fp32 (then its magnitudes are too)
+    #pragma unroll
+    for (int n = 0; n < NT; ++n)
+      #pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (8 * n + 2 * j + e < P.g) { best = fmaxf(best, c[n][2 * r + e]); mag = m[n][2 * r + e] < INFINITY ? fmaxf(mag, m[n][2 * r + e]) : INFINITY; }
+    #pragma unroll
+    for (int d = 1; d < 4; d <<= 1) { best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d)); mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, d)); }
+    const int i = g8 + 8 * r, page = __shfl_sync(0xffffffffu, mine, i);
+    if (j == 0 && b0 + i < n_cand)
+      P.approx[((size_t)row * P.R.kvh + h) * P.R.blocks + b0 + i] = page < 0 ? make_float2(0.f, -1.f) : mag < INFINITY ? make_float2(best, mag) : make_float2(0.f, INFINITY);
   }
 }
 
-// The choice.  The highest keys' range is cut into 2,048 bins at a time, from the highest bit in which the keys differ on: the bin that holds the last place, then, where it holds
-// few keys, the place in it by counting for each how many come before it; otherwise its bins in turn.  Keys of equal height are taken from the lowest block on.
-// Then one walk writes the chosen blocks in rising order.
-constexpr int CT = 512, BINS = 2048, LIST = 256;
+// Bits of a number as an unsigned integer of the same order, above 1; 1 for what is not a number.
+__device__ __forceinline__ u64 key_of(double x) {
+  if (x != x) return 1ull;
+  const long long b = __double_as_longlong(x + 0.0);                    // -0 counts as 0
+  return b < 0 ? ~(u64)b : (u64)b | 0x8000000000000000ull;
+}
+__device__ __forceinline__ uint32_t key_of(float x) {                  // finite; never 0
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float float_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+constexpr int CT = 512, WARPS = CT / 32, PER = 8, BINS = 2048, LIST = 256;     // threads; blocks a thread keeps in registers
+constexpr unsigned ALL = 0xffffffffu;
+struct Shared {
+  uint4 range[WARPS];                        // of each warp: highest and lowest key, number of keys, largest sum of magnitudes
+  alignas(16) int hist[BINS];                // zero between its uses
+  u64 list[LIST], hi[WARPS], lo[WARPS], cut;
+  int warps[WARPS], bin, left, count, n, at[LIST];
+};
+static_assert(BINS == 4 * CT && WARPS == 16, "four bins a thread; half a warp looks at all warps");
+
+// What the warps in front of this one hold, and all of them: v of every warp in sh.warps.
+__device__ __forceinline__ int ahead_of(const Shared& sh, int warp, int lane) { return __reduce_add_sync(ALL, lane < warp ? sh.warps[lane & 15] : 0); }
+__device__ __forceinline__ int of_all(const Shared& sh, int lane) { return __reduce_add_sync(ALL, lane < WARPS ? sh.warps[lane & 15] : 0); }
+__device__ __forceinline__ int upto_lane(int v, int lane) {             // sum of the lanes up to this one
+  #pragma unroll
+  for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(ALL, v, d); if (lane >= d) v += o; }
+  return v;
+}
+
+// The bin that holds the `left`-th highest of the keys counted in sh.hist (zero again behind it), and how many of its keys are among the first `left`.
+__device__ __forceinline__ int border_bin(Shared& sh, int& left) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __syncthreads();
+  int4* h4 = reinterpret_cast<int4*>(sh.hist) + (BINS / 4 - 1 - tid);   // thread t: bins BINS - 1 - 4t and the three below
+  const int4 c = *h4;
+  *h4 = make_int4(0, 0, 0, 0);
+  const int c4[4] = {c.w, c.z, c.y, c.x}, mine = c.x + c.y + c.z + c.w, upto = upto_lane(mine, lane);
+  if (lane == 31) sh.warps[warp] = upto;
+  __syncthreads();
+  int above = ahead_of(sh, warp, lane) + upto - mine;
+  #pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (above < left && above + c4[e] >= left) { sh.bin = BINS - 1 - 4 * tid - e; sh.left = left - above; sh.count = c4[e]; }
+    above += c4[e];
+  }
+  __syncthreads();
+  left = sh.left;
+  return sh.bin;
+}
+
+// The `left`-th highest of the n 64-bit keys (0: no key), and in `left` how many keys of its height are among the first `left`; all keys: 0.  The keys' range is cut into
+// 2,048 bins at a time, from the highest bit in which they differ on.
+__device__ u64 border(Shared& sh, const u64* keys, int n, int& left) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  u64 hi = 0, lo = ~0ull;
+  int count = 0;
+  for (int i = tid; i < n; i += CT) { const u64 k = keys[i]; if (k) { hi = k > hi ? k : hi; lo = k < lo ? k : lo; ++count; } }
+  #pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    const u64 a = __shfl_xor_sync(ALL, hi, d), b = __shfl_xor_sync(ALL, lo, d);
+    hi = a > hi ? a : hi; lo = b < lo ? b : lo;
+  }
+  count = __reduce_add_sync(ALL, count);
+  if (lane == 0) { sh.hi[warp] = hi; sh.lo[warp] = lo; sh.warps[warp] = count; }
+  __syncthreads();
+  for (int i = 0; i < WARPS; ++i) { hi = sh.hi[i] > hi ? sh.hi[i] : hi; lo = sh.lo[i] < lo ? sh.lo[i] : lo; }
+  count = of_all(sh, lane);
+  __syncthreads();
+  if (count <= left) return 0;
+  int top = hi == lo ? 0 : 64 - __clzll((long long)(hi ^ lo));          // the keys that are still looked at have `fixed` from bit `top` on
+  u64 fixed = top < 64 ? hi >> top : 0ull;
+  while (top > 0) {
+    const int shift = max(0, top - 11);
+    for (int i = tid; i < n; i += CT) {
+      const u64 k = keys[i];
+      if (k && (top < 64 ? k >> top : 0ull) == fixed) atomicAdd(&sh.hist[(int)(k >> shift) & ((1 << (top - shift)) - 1)], 1);
+    }
+    fixed = fixed << (top - shift) | (u64)border_bin(sh, left);
+    top = shift;
+  }
+  return fixed;
+}
+
+// fp64 score of block b as a key, by one warp; 0 without a page.  Eight heads at a time, whose sums are folded over the warp together: at each step a lane gives
+// away half of what it holds.
+template <int HD, bool BF> __device__ u64 exact_key(const SelectP& P, const Place& w, int row, int h, int b, int lane) {
+  constexpr int C = HD / 32, GP = 8;
+  const int page = page_of(P.R, w.seq, b);
+  if (page < 0) return 0ull;
+  const uint32_t* src = reinterpret_cast<const uint32_t*>(P.kmean + ((size_t)page * P.R.kvh + h) * HD + C * lane);
+  uint32_t u[C / 2];
+  #pragma unroll
+  for (int e = 0; e < C / 2; ++e) u[e] = src[e];
+  u64 best = 1ull;
+  for (int g0 = 0; g0 < P.g; g0 += GP) {
+    double s[GP];
+    #pragma unroll
+    for (int i = 0; i < GP; ++i) {
+      const uint32_t* qp = reinterpret_cast<const uint32_t*>(P.q + row * P.qs + (size_t)(h * P.g + min(g0 + i, P.g - 1)) * HD + C * lane);
+      s[i] = 0.0;
+      #pragma unroll
+      for (int e = 0; e < C / 2; ++e) {
+        const float2 x = unpack16<BF>(u[e]), y = unpack16<BF>(qp[e]);
+        s[i] = fma((double)x.x, (double)y.x, s[i]); s[i] = fma((double)x.y, (double)y.y, s[i]);
+      }
+    }
+    #pragma unroll
+    for (int d = 16, c = GP / 2; c >= 1; d >>= 1, c >>= 1) {            // 8 -> 4 -> 2 -> 1 sums a lane
+      const bool up = (lane & d) != 0;
+      #pragma unroll
+      for (int i = 0; i < GP / 2; ++i)
+        if (i < c) { const double give = up ? s[i] : s[i + c], keep = up ? s[i + c] : s[i]; s[i] = keep + __shfl_xor_sync(ALL, give, d); }
+    }
+    double t = s[0];                                                    // head g0 + lane / 4, repeated heads among them
+    t += __shfl_xor_sync(ALL, t, 2);
+    t += __shfl_xor_sync(ALL, t, 1);
+    const u64 k = key_of(t);
+    best = k > best ? k : best;
+  }
+  #pragma unroll
+  for (int d = 16; d >= 4; d >>= 1) { const u64 o = __shfl_xor_sync(ALL, best, d); best = o > best ? o : best; }
+  return best;
+}
+
+// The choice, a block a (row, kv-head).
+template <int HD, bool BF>
 __global__ void __launch_bounds__(CT) paged_choose_kernel(const SelectP P) {
-  __shared__ unsigned long long s_hi[CT / 32], s_lo[CT / 32], list[LIST], s_cut;
-  __shared__ int hist[BINS], warps[CT / 32], s_bin, s_left, s_count, s_n;
+  __shared__ Shared sh;
   pdl_wait();
   pdl_launch();
   const int row = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const size_t pair = (size_t)row * P.R.kvh + h;
+  const float2* approx = P.approx + pair * P.R.blocks;
+  u64* exact = P.exact + pair * P.R.blocks;
+  int* ids = P.ids + pair * P.take;
+  // Block i0 + PER tid + e of the scores is x[e].  Up to PER * CT blocks are read once, beside the row's place, and stay; more are read again for each walk.
+  float2 x[PER];
+  auto read = [&](int i0, int end) {
+    #pragma unroll
+    for (int e = 0; e < PER; ++e) { const int i = i0 + PER * tid + e; x[e] = i < end ? approx[i] : make_float2(0.f, -1.f); }
+  };
+  read(0, P.R.blocks - 1);
+  reinterpret_cast<int4*>(sh.hist)[tid] = make_int4(0, 0, 0, 0);
+  if (tid == 0) sh.n = 0;
   const Place w = place_of(P.R, row);
   if (w.seq < 0) return;
-  const size_t pair = (size_t)row * P.R.kvh + h;
-  const unsigned long long* keys = P.keys + pair * P.R.blocks;
-  int* ids = P.ids + pair * P.take;
   const int last = w.vis > 0 ? (w.vis - 1) >> P.R.lp : -1, n = last > 0 ? last : 0;
-
-  // ---- highest and lowest candidate, and how many there are
-  unsigned long long hi = 0, lo = ~0ull;
+  #pragma unroll
+  for (int e = 0; e < PER; ++e) if (PER * tid + e >= n) x[e] = make_float2(0.f, -1.f);       // behind the candidates nothing has been written
+  auto each = [&](auto f) {
+    for (int i0 = 0; i0 < n; i0 += PER * CT) {
+      if (n > PER * CT) read(i0, n);
+      #pragma unroll
+      for (int e = 0; e < PER; ++e) f(i0 + PER * tid + e, x[e]);
+    }
+  };
+  // ---- the scores' range, the largest sum of magnitudes
+  uint32_t khi = 0, klo = ALL, big = 0;
   int count = 0;
-  #pragma unroll 4
-  for (int i = tid; i < n; i += CT) { const unsigned long long k = keys[i]; if (k) { hi = k > hi ? k : hi; lo = k < lo ? k : lo; ++count; } }
-  #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) {
-    const unsigned long long a = __shfl_xor_sync(0xffffffffu, hi, d), b = __shfl_xor_sync(0xffffffffu, lo, d);
-    hi = a > hi ? a : hi; lo = b < lo ? b : lo; count += __shfl_xor_sync(0xffffffffu, count, d);
-  }
-  if (lane == 0) { s_hi[warp] = hi; s_lo[warp] = lo; warps[warp] = count; }
+  each([&](int, const float2& f) {
+    if (f.y >= 0.f) {
+      const uint32_t k = key_of(f.x);
+      khi = max(khi, k); klo = min(klo, k); ++count;
+      big = max(big, __float_as_uint(f.y));                             // not negative: sorts like its bits
+    }
+  });
+  khi = __reduce_max_sync(ALL, khi); klo = __reduce_min_sync(ALL, klo); count = __reduce_add_sync(ALL, count); big = __reduce_max_sync(ALL, big);
+  if (lane == 0) sh.range[warp] = make_uint4(khi, klo, (uint32_t)count, big);
   __syncthreads();
-  count = 0;
-  #pragma unroll
-  for (int i = 0; i < CT / 32; ++i) { hi = s_hi[i] > hi ? s_hi[i] : hi; lo = s_lo[i] < lo ? s_lo[i] : lo; count += warps[i]; }
-  __syncthreads();
+  const uint4 r = sh.range[lane & 15];
+  khi = __reduce_max_sync(ALL, r.x); klo = __reduce_min_sync(ALL, r.y); big = __reduce_max_sync(ALL, r.w);
+  count = __reduce_add_sync(ALL, lane < WARPS ? (int)r.z : 0);
+  // the sum of magnitudes is itself rounded; products below fp32's range (bf16) may count as zero
+  const double e2 = 2.0 * ((HD * 0x1p-21) * 1.01 * (double)__uint_as_float(big) + HD * 0x1p-120);
+  const bool wild = !(e2 < (double)INFINITY), all = count <= P.take - 1;                     // all: no more candidates than places
 
-  // ---- the border: keys above `cut` are taken, and of those equal to it the first `left`
-  unsigned long long cut = 0;
-  int left = P.take - 1;
-  if (count > left && hi == lo) cut = hi;                               // all alike
-  else if (count > left) {
-    int top = 64 - __clzll((long long)(hi ^ lo));                       // the keys that are still looked at have `fixed` from bit `top` on
-    unsigned long long fixed = top < 64 ? hi >> top : 0ull;
-    auto looked = [&](unsigned long long k) { return k && (top < 64 ? k >> top : 0ull) == fixed; };
-    for (;;) {
-      const int shift = max(0, top - 11);
-      for (int i = tid; i < BINS; i += CT) hist[i] = 0;
-      if (tid == 0) s_n = 0;
-      __syncthreads();
-      for (int i = tid; i < n; i += CT) {
-        const unsigned long long k = keys[i];
-        if (looked(k)) atomicAdd(&hist[(int)(k >> shift) & ((1 << (top - shift)) - 1)], 1);
-      }
-      __syncthreads();
-      // thread t has bins BINS - 1 - 4t and the three below: how many keys lie above them
-      int c4[4], mine = 0;
-      #pragma unroll
-      for (int e = 0; e < 4; ++e) { c4[e] = hist[BINS - 1 - 4 * tid - e]; mine += c4[e]; }
-      int upto = mine;
-      #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
-      if (lane == 31) warps[warp] = upto;
-      __syncthreads();
-      for (int i = 0; i < warp; ++i) upto += warps[i];
-      int above = upto - mine;
-      #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (above < left && above + c4[e] >= left) { s_bin = BINS - 1 - 4 * tid - e; s_left = left - above; s_count = c4[e]; }
-        above += c4[e];
-      }
-      __syncthreads();
-      left = s_left;
-      fixed = fixed << (top - shift) | (unsigned long long)s_bin;
-      top = shift;
-      const int in_bin = s_count;
-      if (shift == 0) { cut = fixed; break; }                           // equal keys
-      if (in_bin <= LIST) {
-        for (int i = tid; i < n; i += CT) { const unsigned long long k = keys[i]; if (looked(k)) list[atomicAdd(&s_n, 1)] = k; }
-        __syncthreads();
-        if (tid < in_bin) {                                             // the `left`-th of the list from the top; of equal keys any thread may say it
-          const unsigned long long k = list[tid];
-          int more = 0, same = 0;
-          for (int i = 0; i < in_bin; ++i) { more += list[i] > k; same += list[i] == k; }
-          if (more < left && more + same >= left) { s_cut = k; s_left = left - more; }
-        }
-        __syncthreads();
-        cut = s_cut; left = s_left;
-        break;
-      }
-      __syncthreads();
+  // ---- the bin that holds the border, and what may be on either side of it
+  double lo = -INFINITY, hi = INFINITY;                                 // scored in fp64: what is neither above hi nor below lo
+  if (!wild && !all) {
+    const float flo = float_of(klo), fhi = float_of(khi), scale = (float)BINS / (fhi - flo);
+    lo = (double)flo - e2; hi = (double)fhi + e2;
+    if (fhi - flo < INFINITY && scale < INFINITY) {                     // else all are unsure: scores that are as good as equal, or a range beyond fp32
+      each([&](int, const float2& f) { if (f.y >= 0.f) atomicAdd(&sh.hist[min(BINS - 1, (int)((f.x - flo) * scale))], 1); });
+      int left = P.take - 1;
+      const double bin = (double)border_bin(sh, left), step = 1.0 / (double)scale;
+      // a score's bin is rounded by less than 2^-9 of a bin
+      lo = fmax((double)flo, (double)flo + (bin - 0.01) * step) - e2; hi = fmin((double)fhi, (double)flo + (bin + 1.01) * step) + e2;
     }
   }
-  __syncthreads();
-  // ---- one walk in rising order, four blocks a thread
-  int at = 0, equal = 0;                                                // taken so far; keys equal to the border so far
-  for (int i0 = 0; i0 < n; i0 += 4 * CT) {
-    unsigned long long k4[4];
-    int mine = 0;                                                       // keys above the border, and equal ones << 16
-    #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = i0 + 4 * tid + e;
-      k4[e] = i < n ? keys[i] : 0ull;
-      mine += k4[e] > cut ? 1 : k4[e] && k4[e] == cut ? 1 << 16 : 0;
-    }
-    int upto = mine;
-    #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
-    if (lane == 31) warps[warp] = upto;
+  auto unsure = [&](const float2& f) { return f.y >= 0.f && !((double)f.x > hi) && !((double)f.x < lo); };
+  // ---- the unsure ones: how many, which
+  int sure = 0, many = 0;
+  if (!all) {
+    each([&](int i, const float2& f) {
+      if (unsure(f)) { const int at = atomicAdd(&sh.n, 1); if (at < LIST) sh.at[at] = i; }
+      else if (f.y >= 0.f && (double)f.x > hi) ++sure;
+    });
+    sure = __reduce_add_sync(ALL, sure);
+    if (lane == 0) sh.warps[warp] = sure;
     __syncthreads();
-    int before = upto - mine, all = 0;
+    sure = of_all(sh, lane);
+    many = sh.n;
+  }
+  int left = P.take - 1 - sure;                                         // places for the unsure ones
+  u64 cut = 0;                                                          // of these: above `cut`, and the first `left` equal to it
+  const bool need = !all && many > left, listed = need && many <= LIST && n <= 32 * BINS;
+  if (listed) {
+    for (int i = warp; i < many; i += WARPS) { const u64 k = exact_key<HD, BF>(P, w, row, h, sh.at[i], lane); if (lane == 0) sh.list[i] = k; }
+    __syncthreads();
+    if (tid < many) {                                                   // how many come before this one: the higher, and of equal ones the lower blocks
+      const u64 k = sh.list[tid];
+      const int at = sh.at[tid];
+      int before = 0;
+      for (int i = 0; i < many; ++i) before += sh.list[i] > k || (sh.list[i] == k && sh.at[i] < at);
+      if (before < left) atomicOr(&sh.hist[at >> 5], 1 << (at & 31));   // a bit for each block
+    }
+  } else if (need) {
+    for (int i = warp; i < n; i += WARPS) {
+      u64 k = 0;
+      if (unsure(approx[i])) k = exact_key<HD, BF>(P, w, row, h, i, lane);
+      if (lane == 0) exact[i] = k;
+    }
+    __syncthreads();
+    cut = border(sh, exact, n, left);
+  }
+  __syncthreads();
+  // ---- one walk in rising order, PER blocks a thread
+  int at = 0, equal = 0;                                                // taken so far; keys equal to the border so far
+  for (int i0 = 0; i0 < n; i0 += PER * CT) {
+    if (n > PER * CT) read(i0, n);
+    int what[PER], mine = 0;                                            // 1: taken; 1 << 16: equal to the border
     #pragma unroll
-    for (int i = 0; i < CT / 32; ++i) { const int v = warps[i]; if (i < warp) before += v; all += v; }
+    for (int e = 0; e < PER; ++e) {
+      const int i = i0 + PER * tid + e;
+      const float2 f = x[e];
+      what[e] = 0;
+      if (f.y >= 0.f) {
+        if (all || (double)f.x > hi) what[e] = 1;
+        else if (unsure(f)) {
+          if (!need) what[e] = 1;
+          else if (listed) what[e] = (sh.hist[i >> 5] >> (i & 31)) & 1;
+          else { const u64 k = exact[i]; what[e] = k > cut ? 1 : k && k == cut ? 1 << 16 : 0; }
+        }
+      }
+      mine += what[e];
+    }
+    const int upto = upto_lane(mine, lane);
+    if (lane == 31) sh.warps[warp] = upto;
+    __syncthreads();
+    const int before = ahead_of(sh, warp, lane) + upto - mine, total = of_all(sh, lane);
     int a = before & 0xffff, e0 = equal + (before >> 16);
     #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const bool eq = k4[e] && k4[e] == cut, take = k4[e] > cut || (eq && e0 < left);
-      if (take) ids[at + a + min(e0, left) - min(equal, left)] = i0 + 4 * tid + e;
-      a += k4[e] > cut; e0 += eq;
+    for (int e = 0; e < PER; ++e) {
+      if (what[e] == 1 || (what[e] > 1 && e0 < left)) ids[at + a + min(e0, left) - min(equal, left)] = i0 + PER * tid + e;
+      a += what[e] & 1; e0 += what[e] >> 16;
     }
-    at += (all & 0xffff) + min(equal + (all >> 16), left) - min(equal, left);
-    equal += all >> 16;
-    __syncthreads();
+    at += (total & 0xffff) + min(equal + (total >> 16), left) - min(equal, left);
+    equal += total >> 16;
+    if (i0 + PER * CT < n) __syncthreads();
   }
   if (tid == 0 && last >= 0) ids[at] = last;
   if (last >= 0) ++at;
   for (int i = at + tid; i < P.take; i += CT) ids[i] = -1;
 }
 
+template <int HD, bool BF> int launch(const SelectP& P, cudaStream_t st) {
+  if (P.R.blocks > 1) {
+    auto score = P.g <= 8 ? paged_score_kernel<HD, BF, 1> : paged_score_kernel<HD, BF, 2>;
+    constexpr int per = 16 * SCORE_WARPS;
+    if (int rc = launch_pdl("paged_score_kernel", score, dim3((unsigned)((P.R.blocks - 1 + per - 1) / per), (unsigned)P.R.kvh, (unsigned)P.rows), SCORE_WARPS * 32, 0, st, P))
+      return rc;
+  }
+  return launch_pdl("paged_choose_kernel", paged_choose_kernel<HD, BF>, dim3((unsigned)P.R.kvh, (unsigned)P.rows), CT, 0, st, P);
+}
+
 }  // namespace
 }  // namespace paged
 
-size_t paged_select_bytes(const yskn_paged_cache& c, int rows, int blocks) { return (size_t)rows * c.kvh * blocks * 8; }
+size_t paged_select_bytes(const yskn_paged_cache& c, int rows, int blocks) { return (size_t)rows * c.kvh * blocks * 16; }
 
 int launch_paged_select(const yskn_paged_cache& c, const yskn_paged_rows& r, const yskn_paged_select_args& a, cudaStream_t st) {
   using namespace paged;
+  const size_t n = (size_t)r.rows * c.kvh * r.blocks;
+  SelectP P{rows_of(c, r, 0), r.rows, a.nh / c.kvh, a.nh, static_cast<const uint16_t*>(a.q), (long long)a.q_stride, static_cast<const uint16_t*>(c.kmean),
+            static_cast<float2*>(a.workspace), reinterpret_cast<u64*>(static_cast<float2*>(a.workspace) + n), a.take, a.ids};
   const bool bf = c.dtype == YSKN_KV4_BF16;
-  const int g = a.nh / c.kvh;
-  SelectP P{rows_of(c, r, 0), r.rows, g, a.nh, static_cast<const uint16_t*>(a.q), (long long)a.q_stride, static_cast<const uint16_t*>(c.kmean),
-            static_cast<unsigned long long*>(a.workspace), a.take, a.ids};
-  auto score = c.hd == 256 ? (bf ? paged_score_kernel<256, true> : paged_score_kernel<256, false>)
-                           : (bf ? paged_score_kernel<128, true> : paged_score_kernel<128, false>);
-  if (r.blocks > 1) {
-    // blocks of a warp: as many as leave two CTAs an SM, since a CTA's start (its queries as fp64) costs what eight blocks do
-    int per = 4;
-    while (per < 64 && (long long)r.rows * c.kvh * ((r.blocks - 1) / (SCORE_WARPS * 2 * per)) >= 2 * SMS) per *= 2;
-    const int cta = SCORE_WARPS * per;
-    if (int rc = launch_pdl("paged_score_kernel", score, dim3((unsigned)((r.blocks - 1 + cta - 1) / cta), (unsigned)c.kvh, (unsigned)r.rows), SCORE_WARPS * 32, 0, st, P, per))
-      return rc;
-  }
-  return launch_pdl("paged_choose_kernel", paged_choose_kernel, dim3((unsigned)c.kvh, (unsigned)r.rows), CT, 0, st, P);
+  return c.hd == 256 ? (bf ? launch<256, true>(P, st) : launch<256, false>(P, st)) : (bf ? launch<128, true>(P, st) : launch<128, false>(P, st));
 }
 
 }  // namespace kv4
