@@ -40,6 +40,7 @@ struct AttnP {
   int shared; const int* ids; int take;
   int2* span; float2* ml; float* pacc;       // first and last CTA of a pair; its pieces: maxima and sums, O
   const float2* qml; const float* qacc; int splits;     // partials over the shared prefix
+  int beside;                                // the launch in front is the prefix kernel of this call
 };
 
 template <int HD, int NT> struct Lay {
@@ -96,7 +97,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     asm volatile("prefetch.tensormap [%0];" ::"l"(&mapV) : "memory");
   }
   __syncthreads();
-  pdl_wait();
+  // Behind the prefix kernel there is nothing to wait for: it lets this one start when all of its blocks have seen what lies in front of it finished, and this one
+  // reads nothing that it writes, so the two run side by side where there is room.  The wait comes at the end: the merge waits for this grid, and thereby for both.
+  if (!P.beside) pdl_wait();
   pdl_launch();
 
   // ---- the line: first[r] = tiles of one kv-head ahead of row r.  Every warp finds it for itself (all write the same): no barrier between the positions and the first copy
@@ -118,7 +121,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     __syncwarp();
   }
   const int kvh = P.R.kvh, total = first[ROWS] * kvh, grid = min((int)gridDim.x, total), cta = (int)blockIdx.x;       // every CTA below `grid` has a tile at least
-  if (cta >= grid) return;
+  if (cta >= grid) { if (P.beside) pdl_wait(); return; }
   const int u0 = (int)((long long)total * cta / grid), u1 = (int)((long long)total * (cta + 1) / grid);
 
   // The row that holds unit u: the last whose first unit is not behind it
@@ -200,6 +203,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
       for (int it = max(0, issued - NSLOT); it < issued; ++it) bar_wait(b_full + 8 * (it % NSLOT), (it / NSLOT) & 1);
       for (int it = max(0, queries - 2); it < queries; ++it) bar_wait(b_qfull + 8 * (it & 1), (it >> 1) & 1);
     }
+    if (P.beside) pdl_wait();
     return;
   }
 
@@ -380,6 +384,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     t0 = 0;
     if (++head == kvh) { head = 0; do ++row; while (row < P.rows && first[row + 1] == first[row]); nt = row < P.rows ? first[row + 1] - first[row] : 1; }
   }
+  if (P.beside) pdl_wait();
 }
 
 // Joins what the parts of a (row, head) hold: partials over the shared prefix, then pieces of CTAs.  W warps a (row, head): each looks at all parts' maxima and sums by itself,
@@ -533,7 +538,7 @@ int launch_paged_attention(const yskn_paged_cache& c, const yskn_paged_rows& r, 
     const size_t part = (size_t)first * splits * a.nh;
     AttnP P{rows_of(c, r, first), rows, g, a.nh, static_cast<const uint16_t*>(a.q) + first * a.q_stride, (long long)a.q_stride, a.qscale * LOG2E,
             static_cast<uint16_t*>(a.o16) + (size_t)first * a.nh * c.hd, splits > 0 ? a.shared : 0, a.ids ? a.ids + (size_t)first * c.kvh * a.take : nullptr, a.take,
-            w.span, w.ml, w.pacc, w.qml + part, w.qacc + part * c.hd, splits};
+            w.span, w.ml, w.pacc, w.qml + part, w.qacc + part * c.hd, splits, splits > 0 && first == 0 ? 1 : 0};
     if (int rc = c.hd == 256 ? dispatch<256>(c, P, st) : dispatch<128>(c, P, st)) return rc;
     // few rows: their parts are many, a block adds them up together; many rows: few parts each, a warp does
     const bool bf = c.dtype == YSKN_KV4_BF16, few = (long long)rows * a.nh <= 2 * SMS;
