@@ -440,8 +440,8 @@ typedef struct yskn_paged_rows {
  * (c < rd/2) turn by entry [pos][c] of `rope`, (cos, sin) pairs fp32 [rope_rows][rd/2] as yskn_kv4_rope_table writes them, in fp32, rounded once;
  * rd a multiple of 16, at most hd, 0: no rotation.  All rows have the cache's type; pointers and strides are multiples of 16 bytes.
  * A row at a position that has no page (or, with rd > 0, no entry of the table: negative, or beyond rope_rows) is left out, its query too where the position
- * has no entry.  With kmean the mean key (fp32 sum) of each page whose last row is among these rows is written by a second launch.
- * Two rows of one call must not share a place. */
+ * has no entry.  With kmean the mean key (fp32 sum) of each page whose last row is among these rows is written too.
+ * Two rows of one call must not share a place, and rows of one call that go to the same page belong to one sequence. */
 typedef struct yskn_paged_append_args {
   const void* k_in; const void* v_in; const void* q_in; void* q_out;
   int64_t k_stride, v_stride, q_stride;
