@@ -5,7 +5,10 @@
 // Mean of a page: fp32 sum of its `page` rows in a fixed order, times 1 / page (a power of two, exact), rounded once.
 //
 // Bound: bytes.  Every row is read and written once, 16 bytes a lane; a warp holds whole heads (hd 256: one, hd 128: two), so the other channel of a pair
-// is in another lane of the same warp and comes by a shuffle.
+// is in another lane of the same warp and comes by a shuffle.  8,192 rows of 24 + 2 * 4 heads of 256 channels: 52.6 us, 5.2 TB/s of 6.6 that a copy has.  What that
+// took: nobody reads the inputs again, and of a prompt nobody the rows before L2 has let them go, so both pass as streaming data (57.2 us without either hint, 56.7 with
+// one); 32 warps an SM with four loads each (two loads a lane 71 us, eight 76; a loop over items with the next one's loads ahead 65); the means' blocks first, since
+// they bring the keys into L2 (last 61 us, between the others 64).
 //
 // The means are taken in the same launch, by blocks of their own: of a page's rows those that this call brings are turned again from the call's inputs, as their
 // places in the cache are being written at the same time, and the others are read from the cache.  A launch behind the first one took a
@@ -142,7 +145,7 @@ __global__ void __launch_bounds__(256, 4) paged_append_kernel(const AppendP P) {
     if (vh[i] >= 0) {
       const uint16_t* src = h < nq ? P.q_in + row * P.qs + (size_t)h * HD : h < nq + kvh ? P.k_in + row * P.ks + (size_t)(h - nq) * HD
                                                                                        : P.v_in + row * P.vs + (size_t)(h - nq - kvh) * HD;
-      x[i] = *reinterpret_cast<const uint4*>(src + ch);
+      x[i] = __ldcs(reinterpret_cast<const uint4*>(src + ch));
     }
   }
   const int s = P.R.seq[row], pos = P.R.pos[row];
@@ -171,7 +174,7 @@ __global__ void __launch_bounds__(256, 4) paged_append_kernel(const AppendP P) {
       const size_t at = (((size_t)page * kvh + (h < kvh ? h : h - kvh)) << P.R.lp) + (pos & (P.R.page - 1));
       dst = (h < kvh ? P.k : P.v) + at * HD;
     }
-    *reinterpret_cast<uint4*>(dst + ch) = y;
+    __stcs(reinterpret_cast<uint4*>(dst + ch), y);
   }
 }
 
