@@ -7,7 +7,9 @@
 //
 // A pair of CTAs (a cluster of two, cta_group::2) takes 256 (row, head) pairs of one kv-head, 128 each, and one run of the tokens in tiles of 128.  Per CTA:
 //   warps 0-7   two warpgroups that take the tiles in turn, a thread a row: scores from tensor memory, running maximum, weights back over the scores just read
-//   warp 8      TMA: its half of every K tile (64 tokens) and V tile (HD/2 channels), a box of min(page, 64) rows x 64 channels a copy, three and two stages
+//   warps 8, 10 TMA: its half of every K tile (64 tokens), of every V tile (HD/2 channels), a box of min(page, 64) rows x 64 channels a copy, three and two stages.  A
+//               warp each, since a stage of V is free two tiles later than one of K: asked for in turn, K came a tile ahead of its use and the tensor pipe waited 780
+//               cycles a tile for it
 //   warp 9      (leader) issues S = Q K^T (M256 N128) into one of two buffers of tensor memory and O += P V (M256 N = HD, P from tensor memory)
 // Each CTA stages half a tile because an SM takes in 40 to 50 bytes a clock from L2, and a whole tile a CTA would want 64.  S of the next tile but one is issued
 // behind P V of this one, so the tensor pipe works while the weights are computed; O is rescaled only where a maximum has grown by more than 2^8.
@@ -124,7 +126,6 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
                  b_pready = b0 + 144, b_q = b0 + 160;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::OFF_BAR + 168);
   volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::OFF_BAR + 172);
-  int* s_src = reinterpret_cast<int*>(smem + L::OFF_BAR + 176);
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::NK; ++i) { bar_init(b_kfull + 8 * i, 1); bar_init(b_kempty + 8 * i, 1); }
     for (int i = 0; i < L::NV; ++i) { bar_init(b_vfull + 8 * i, 1); bar_init(b_vempty + 8 * i, 1); }
@@ -133,7 +134,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
       bar_init(b_phalf + 8 * i, 2 * nquad); bar_init(b_pready + 8 * i, 2 * nquad);          // the warps with queries of the tile's warpgroup, both CTAs
     }
     bar_init(b_q, 2 * SW);
-    *s_abort = 0; *s_src = 0x7fffffff;
+    *s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (threadIdx.x < 128) reinterpret_cast<volatile uint32_t*>(smem + L::OFF_XCH + 4 * 128 * 4)[threadIdx.x] = 0;
@@ -150,53 +151,48 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
   pdl_wait();
   pdl_launch();
 
-  // ---- the first row that has the whole prefix: its table names the pages.  Both CTAs of a pair find the same
-  for (int r0 = 0; r0 < P.rows; r0 += THREADS) {
-    const int r = r0 + (int)threadIdx.x;
-    const bool found = r < P.rows && place_of(P.R, r).vis >= P.shared;
-    if (found) atomicMin(s_src, r);
-    if (__syncthreads_or(found)) break;
-  }
-  const int src = *s_src;
   const int kvh = blockIdx.z, split = blockIdx.y, row0 = (int)blockIdx.x * P.tpc;
-  const int j0 = split * P.per, n = src == 0x7fffffff ? 0 : min(P.tiles, j0 + P.per) - j0;
+  const int j0 = split * P.per, n = min(P.tiles, j0 + P.per) - j0;
 
-  int k_issued = 0, v_issued = 0;                                      // stages that the producer has asked for
+  int issued = 0;                                                      // stages that a producer has asked for
   auto fail = [&]() { atomicExch(&g_prefix_status, 8); *s_abort = 1; };
 
-  auto role_producer = [&]() {
+  auto role_producer = [&](const bool is_v) {
     const int lc = min(P.R.lp, 6), chunk = 1 << lc, npt = BN >> lc;    // rows of a box; boxes of a tile's tokens
-    const int seq = P.R.seq[src], none = (P.R.pages * P.R.kvh) << P.R.lp;
-    auto row_at = [&](int ci) {                                        // chunk ci of the prefix as a row of the arrays
-      const int tok = ci << lc;
-      if (tok >= P.shared) return none;
-      const int pg = page_of(P.R, seq, tok >> P.R.lp);
-      return pg < 0 ? none : ((pg * P.R.kvh + kvh) << P.R.lp) + (tok & (P.R.page - 1));
-    };
-    const uint32_t lead_k = leader_addr(b_kfull), lead_v = leader_addr(b_vfull);
-    const int tpb = 32 / npt, npk = npt / 2;
-    int at0 = row_at(j0 * npt + lane), at1 = row_at(j0 * npt + 32 + lane);
-    bool ok = true;
-    for (int i = 0; i < n; ++i) {
-      const int in = i % tpb;
-      if (i > 0 && in == 0) { at0 = at1; at1 = row_at((j0 + i + tpb) * npt + lane); }
-      const int kc = lane / L::KBLK, kb = lane % L::KBLK, vc = lane / L::VBLK, vb = lane % L::VBLK;
-      const int kat = __shfl_sync(0xffffffffu, at0, in * npt + rank * npk + min(kc, npk - 1)), vat = __shfl_sync(0xffffffffu, at0, in * npt + min(vc, npt - 1));
-      const int ks = i % L::NK, vs = i % L::NV;
-      if (i >= L::NK) ok = bar_wait(b_kempty + 8 * ks, (i / L::NK - 1) & 1);
-      ok = __all_sync(0xffffffffu, ok && !*s_abort);
-      if (!ok) break;
-      if (rank == 0 && lane == 0) bar_expect_tx(b_kfull + 8 * ks, 2 * L::K_HALF);
-      ++k_issued;
-      if (kc < npk) tma_pair(sb + L::OFF_K + ks * L::K_HALF + kb * L::K_BLOCK + kc * (chunk * 128), &mapK, 0, kat, kb, lead_k + 8 * ks);
-      if (i >= L::NV) ok = bar_wait(b_vempty + 8 * vs, (i / L::NV - 1) & 1);
-      ok = __all_sync(0xffffffffu, ok && !*s_abort);
-      if (!ok) break;
-      if (rank == 0 && lane == 0) bar_expect_tx(b_vfull + 8 * vs, 2 * L::V_HALF);
-      ++v_issued;
-      if (vc < npt) tma_pair(sb + L::OFF_V + vs * L::V_HALF + vb * L::V_BLOCK + vc * (chunk * 128), &mapV, 0, vat, L::VBLK * rank + vb, lead_v + 8 * vs);
+    const int none = (P.R.pages * P.R.kvh) << P.R.lp;                  // a row outside the arrays: zeros
+    // The first row that has the whole prefix: its table names the pages.  Where no row has, zeros are taken and nothing is kept.
+    int seq = -1;
+    for (int r0 = 0; r0 < P.rows && seq < 0; r0 += 32) {
+      Place w{-1, 0};
+      if (r0 + lane < P.rows) w = place_of(P.R, r0 + lane);
+      const unsigned found = __ballot_sync(0xffffffffu, w.vis >= P.shared);
+      if (found) seq = __shfl_sync(0xffffffffu, w.seq, __ffs(found) - 1);
     }
-    if (!ok && lane == 0) fail();
+    auto row_at = [&](int ci) {                                        // chunk ci of the prefix as a row of the arrays
+      const long long tok = (long long)ci << lc;
+      if (tok >= P.shared || seq < 0) return none;
+      const int pg = page_of(P.R, seq, (int)(tok >> P.R.lp));
+      return pg < 0 ? none : ((pg * P.R.kvh + kvh) << P.R.lp) + (int)(tok & (P.R.page - 1));
+    };
+    const int tpb = 32 / npt, blks = is_v ? L::VBLK : L::KBLK, boxes = is_v ? npt : npt / 2, stages = is_v ? L::NV : L::NK;
+    const int box = lane / blks, blk = lane % blks;                    // this lane's copy: tokens, 64 channels
+    const uint32_t full = is_v ? b_vfull : b_kfull, empty = is_v ? b_vempty : b_kempty, lead = leader_addr(full), bytes = is_v ? L::V_HALF : L::K_HALF;
+    const uint32_t dst = sb + (is_v ? L::OFF_V + blk * L::V_BLOCK : L::OFF_K + blk * L::K_BLOCK) + box * (chunk * 128);
+    const int z = is_v ? L::VBLK * rank + blk : blk, from = (is_v ? 0 : rank * boxes) + min(box, boxes - 1);
+    const CUtensorMap* map = is_v ? &mapV : &mapK;
+    int at0 = row_at(j0 * npt + lane), at1 = at0;                      // 32 boxes, one a lane, and the 32 behind them
+    for (int i = 0; i < n; ++i) {
+      const int in = i % tpb, st = i % stages;
+      if (i > 0 && in == 0) at0 = at1;
+      const int at = __shfl_sync(0xffffffffu, at0, in * npt + from);
+      bool ok = i < stages || bar_wait(empty + 8 * st, (i / stages - 1) & 1);
+      ok = __all_sync(0xffffffffu, ok && !*s_abort);
+      if (!ok) { if (lane == 0) fail(); break; }
+      if (rank == 0 && lane == 0) bar_expect_tx(full + 8 * st, 2 * bytes);
+      ++issued;
+      if (box < boxes) tma_pair(dst + st * bytes, map, 0, at, z, lead + 8 * st);
+      if (in == min(2, tpb - 1)) at1 = row_at((j0 + i - in + tpb) * npt + lane);            // once the stages are full
+    }
   };
 
   auto role_mma = [&]() {
@@ -252,13 +248,20 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
     const int quad = warp & 3, hf = warp >> 2, rho = quad * 32 + lane; // quadrant of tensor memory; warpgroup; row of the tile
     const int row = row0 + rho / G, head = kvh * G + rho % G;
     // ---- queries into the swizzled blocks
-    #pragma unroll 4
-    for (int it = threadIdx.x; it < 128 * (HD / 8); it += 32 * SW) {
-      const int r = it / (HD / 8), w = it % (HD / 8), t = r / G;
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      if (t < P.tpc && row0 + t < P.rows) u = *reinterpret_cast<const uint4*>(P.q + (row0 + t) * P.qs + (size_t)(kvh * G + r - t * G) * HD + 8 * w);
-      u.x ^= P.flip; u.y ^= P.flip; u.z ^= P.flip; u.w ^= P.flip;
-      sts128(sb + (w >> 3) * L::Q_BLOCK + r * 128 + (((w & 7) ^ (r & 7)) << 4), u);
+    {
+      constexpr int N = 128 * (HD / 8) / (32 * SW);                    // 16-byte pieces a thread, all asked for together
+      uint4 u[N];
+      #pragma unroll
+      for (int x = 0; x < N; ++x) {
+        const int it = threadIdx.x + x * 32 * SW, r = it / (HD / 8), w = it % (HD / 8), t = r / G;
+        u[x] = make_uint4(0u, 0u, 0u, 0u);
+        if (t < P.tpc && row0 + t < P.rows) u[x] = *reinterpret_cast<const uint4*>(P.q + (row0 + t) * P.qs + (size_t)(kvh * G + r - t * G) * HD + 8 * w);
+      }
+      #pragma unroll
+      for (int x = 0; x < N; ++x) {
+        const int it = threadIdx.x + x * 32 * SW, r = it / (HD / 8), w = it % (HD / 8);
+        sts128(sb + (w >> 3) * L::Q_BLOCK + r * 128 + (((w & 7) ^ (r & 7)) << 4), make_uint4(u[x].x ^ P.flip, u[x].y ^ P.flip, u[x].z ^ P.flip, u[x].w ^ P.flip));
+      }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
@@ -386,19 +389,18 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
 
   if (warp < SW) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    if (n > 0) role_softmax();
+    role_softmax();
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (n > 0) {
-      if (warp == SW) role_producer();
-      else if (warp == SW + 1 && rank == 0) role_mma();
-    }
+    if (warp == SW) role_producer(false);
+    else if (warp == SW + 2) role_producer(true);
+    else if (warp == SW + 1 && rank == 0) role_mma();
   }
   fence_before();
   __syncthreads();
-  if (warp == SW && rank == 0 && *s_abort) {                           // copies of both CTAs that are still under way land before the pair ends
-    for (int i = max(0, k_issued - L::NK); i < k_issued; ++i) bar_wait(b_kfull + 8 * (i % L::NK), (i / L::NK) & 1);
-    for (int i = max(0, v_issued - L::NV); i < v_issued; ++i) bar_wait(b_vfull + 8 * (i % L::NV), (i / L::NV) & 1);
+  if (rank == 0 && *s_abort) {                                         // copies of both CTAs that are still under way land before the pair ends
+    if (warp == SW) for (int i = max(0, issued - L::NK); i < issued; ++i) bar_wait(b_kfull + 8 * (i % L::NK), (i / L::NK) & 1);
+    if (warp == SW + 2) for (int i = max(0, issued - L::NV); i < issued; ++i) bar_wait(b_vfull + 8 * (i % L::NV), (i / L::NV) & 1);
   }
   __syncwarp();
   cluster_sync_all();                                                  // neither CTA's memory is in use by the other any more
