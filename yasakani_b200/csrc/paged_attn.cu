@@ -15,8 +15,8 @@
 // each for S, share the tile's maxima and weights through shared memory (two named barriers a tile), and take HD / 4 channels each for O, so no warp holds a copy of O.
 // hd 256: one CTA an SM (192 KB in flight); hd 128: two.
 //
-// Tokens that a row does not see: absent blocks are read outside the tensor map (zeros); what a page holds behind the sequence's end is zeroed in
-// shared memory before the product (a weight of 0 times an infinity would be none); scores are masked by selection.
+// Tokens that a row does not see: absent blocks are read outside the tensor map (zeros); what a page holds behind the sequence's end leaves the fragments of V by a mask
+// (a weight of 0 times an infinity would be none; zeroed in shared memory it cost each row's last tile 1 us); scores are masked by selection.
 // Every wait is bounded; one that runs out sets the status word (7) and all warps walk to the end without waiting again.
 #include "paged_common.cuh"
 #include <algorithm>
@@ -306,16 +306,6 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
       // ---- O^T of this warp's channels
       wait(b_full + 8 * vslot, iv / NSLOT);
       const uint32_t sv = sb + vslot * L::HALF;
-      bool whole = true;                                                                    // every row of the tile is a token that the row sees, or came as zeros
-      for (int i = 0; i < npt; ++i) whole &= base_of(i) == 0x7fffffff || base_of(i) + chunk <= w.vis;
-      if (!whole) {
-        for (int i = threadIdx.x; i < TILE * (HD / 8); i += 128) {
-          const int r = i / (HD / 8), cc = i % (HD / 8), ch = r >> lc, rw = r & (chunk - 1);
-          if (base_of(ch) != 0x7fffffff && base_of(ch) + rw >= w.vis)
-            sts128(sv + ch * (chunk * HD * 2) + (cc >> 3) * (chunk * 128) + rw * 128 + (((cc & 7) ^ (rw & 7)) << 4), make_uint4(0u, 0u, 0u, 0u));
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");                        // ahead of the copy that comes next into this half stage
-      }
       compute_sync();
       #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -328,12 +318,16 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
         for (int n = 0; n < NT; ++n) ldm4(sb + L::OFF_P + (buf * NT * 8 + n * 8 + (lane & 7)) * L::PP + (4 * h + (lane >> 3)) * 16, pf[n]);
         #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-          const int t16 = 32 * h + 16 * ks, ch = t16 >> lc, r = (t16 & (chunk - 1)) + (lane & 7) + ((lane >> 4) & 1) * 8;
+          const int t16 = 32 * h + 16 * ks, ch = t16 >> lc, r16 = t16 & (chunk - 1), r = r16 + (lane & 7) + ((lane >> 4) & 1) * 8;
+          // of these 16 tokens the row sees the first n16 (no block: none, and what was read is zero); a lane's registers hold tokens 2j, 2j + 1 and the eight behind them
+          const int n16 = w.vis - base_of(ch) - r16 - 2 * j;
+          const uint32_t keep0 = (n16 > 0 ? 0xffffu : 0u) | (n16 > 1 ? 0xffff0000u : 0u), keep1 = (n16 > 8 ? 0xffffu : 0u) | (n16 > 9 ? 0xffff0000u : 0u);
           #pragma unroll
           for (int y = 0; y < MT; ++y) {
             const int cc = warp * (2 * MT) + 2 * y + ((lane >> 3) & 1);
             uint32_t a[4];
             ldm4t(sv + ch * (chunk * HD * 2) + (cc >> 3) * (chunk * 128) + r * 128 + (((cc & 7) ^ (r & 7)) << 4), a);
+            a[0] &= keep0; a[1] &= keep0; a[2] &= keep1; a[3] &= keep1;
             #pragma unroll
             for (int n = 0; n < NT; ++n) mma<BF>(o[n][y], a, pf[n][2 * ks], pf[n][2 * ks + 1]);
           }
