@@ -476,8 +476,8 @@ typedef struct yskn_paged_attn_args {
   void* workspace; size_t workspace_bytes;
 } yskn_paged_attn_args;
 YSKN_KV4_API int yskn_kv4_paged_attention(const yskn_paged_cache* c, const yskn_paged_rows* r, const yskn_paged_attn_args* a, void* cuda_stream);
-/* Bytes that yskn_kv4_paged_attention over `rows` rows needs with this `shared`, and, where blocks > 0, yskn_kv4_paged_select over a table of so many blocks (the larger
- * of the two); 0 for a shape that is refused. */
+/* Bytes that yskn_kv4_paged_attention over up to `rows` rows needs with up to `shared` shared tokens, and, where blocks > 0, yskn_kv4_paged_select over a table of up to so
+ * many blocks (the larger of the two); 0 for a shape that is refused. */
 YSKN_KV4_API size_t yskn_kv4_paged_workspace_bytes(const yskn_paged_cache* c, int rows, int nh, int shared, int blocks);
 
 #ifdef __cplusplus

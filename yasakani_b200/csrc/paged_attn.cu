@@ -6,7 +6,8 @@
 // tiles are for: S^T[16 tokens x 8 heads] = K Q^T, O^T[16 channels x 8 heads] += V^T P^T, keys and values straight from the swizzled tiles (ldmatrix).
 //
 // Work split.  The tiles of all (row, kv-head) pairs form one line, row after row, which the CTAs of a grid that fills the GPU share out evenly, whatever the lengths
-// are: no CTA has more than one tile above another.  A CTA's run covers parts of one or several pairs.  A pair that lies in one CTA is finished there; of a
+// are.  A pair's start and end cost what a tile does, so in the line it is a step longer than its tiles (64 rows of 1 to 1,500 tokens in four kv-heads: CTAs took
+// 23 to 36 us, by the number of their pairs).  A CTA's run covers parts of one or several pairs.  A pair that lies in one CTA is finished there; of a
 // pair that lies on several each CTA writes (m, l, O) to the piece number (CTA + pair), which is unique because along the line either number only grows, and
 // the merge kernel adds the pieces up.  Every CTA derives the line from the positions itself (a scan over at most ROWS rows).
 //
@@ -102,13 +103,13 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
   if (!P.beside) pdl_wait();
   pdl_launch();
 
-  // ---- the line: first[r] = tiles of one kv-head ahead of row r.  Every warp finds it for itself (all write the same): no barrier between the positions and the first copy
+  // ---- the line: first[r] = steps of one kv-head ahead of row r; a row's are one, without a tile, and its tiles.  Every warp finds it for itself (all write the same): no barrier between the positions and the first copy
   {
     int below = 0;
     for (int r0 = 0; r0 < ROWS; r0 += 32) {
       const int r = r0 + lane;
       int mine = 0;
-      if (r < P.rows) { const Place w = place_of(P.R, r); places[r] = w; mine = tiles_of(P, w); }
+      if (r < P.rows) { const Place w = place_of(P.R, r); places[r] = w; const int nt = tiles_of(P, w); mine = nt > 0 ? nt + 1 : 0; }
       int upto = mine;
       if (r0 < P.rows) {
         #pragma unroll
@@ -120,11 +121,11 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     if (lane == 0) first[ROWS] = below;
     __syncwarp();
   }
-  const int kvh = P.R.kvh, total = first[ROWS] * kvh, grid = min((int)gridDim.x, total), cta = (int)blockIdx.x;       // every CTA below `grid` has a tile at least
+  const int kvh = P.R.kvh, total = first[ROWS] * kvh, grid = min((int)gridDim.x, total), cta = (int)blockIdx.x;       // every CTA below `grid` has a step at least
   if (cta >= grid) { if (P.beside) pdl_wait(); return; }
   const int u0 = (int)((long long)total * cta / grid), u1 = (int)((long long)total * (cta + 1) / grid);
 
-  // The row that holds unit u: the last whose first unit is not behind it
+  // The row that holds step u: the last whose first step is not behind it
   auto row_of = [&](int u) {
     int lo = 0, hi = P.rows - 1;
     while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (first[mid] * kvh <= u) lo = mid; else hi = mid - 1; }
@@ -138,13 +139,14 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     // Boxes come 32 at a time, one a lane, looked up a batch ahead and across the borders of pairs: the lookups' latency (place, chosen block, table) is never
     // waited for.  A box: its row in the arrays, the position of its first token (no token: INT_MAX), its pair.
     struct Box { int at, base, pair; };
-    auto box_of = [&](int u, int j) {                                  // box j of unit u
+    auto box_of = [&](int u, int j) {                                  // box j of step u; of a step without a tile: pair -1
       Box x{none, 0x7fffffff, -1};
       if (u >= u1) return x;
-      const int row = row_of(u), nt = first[row + 1] - first[row], in = u - first[row] * kvh, head = in / nt;
+      const int row = row_of(u), steps = first[row + 1] - first[row], in = u - first[row] * kvh, head = in / steps, t = in - head * steps - 1;
+      if (t < 0) return x;
       const Place w = places[row];
       x.pair = row * kvh + head;
-      const int ci = (in - head * nt) * npt + j;
+      const int ci = t * npt + j;
       int b = -1, sub = 0;
       if (P.ids) {
         const int cpp = P.R.lp - lc, e = ci >> cpp;                    // log2 of a page's boxes; entry
@@ -165,13 +167,14 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     bool ok = *s_abort == 0;
     const int tpb = 32 / npt, jl = lane & (npt - 1), tl = lane / npt;  // tiles of a batch; this lane's box and tile in it
     Box now = box_of(u0 + tl, jl), next = now;
-    for (int u = u0; u < u1 && ok; ++u, ++k) {
+    for (int u = u0; u < u1 && ok; ++u) {
       int i = u - u0;
       if (i > 0 && i % tpb == 0) now = next;
       const bool look = i % tpb == min(3, tpb - 1);                    // for the next batch, once the ring is full
       const int behind = u - i % tpb + tpb + tl;
       i = (i % tpb) * npt + jl;
       const int at = __shfl_sync(0xffffffffu, now.at, i), base = __shfl_sync(0xffffffffu, now.base, i), pr = __shfl_sync(0xffffffffu, now.pair, i);
+      if (pr < 0) { if (look) next = box_of(behind, jl); continue; }
       if (pr != pair) {                                                // queries of the next pair
         pair = pr;
         const int sg = queries;
@@ -196,6 +199,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
         ++issued;
         if (lane < npt) tma_3d(sb + slot * L::HALF + lane * (chunk * HD * 2), v ? &mapV : &mapK, 0, at, 0, b_full + 8 * slot);
       }
+      ++k;
       if (look) next = box_of(behind, jl);
     }
     if (!ok) {                                                         // give up; the copies under way land before the block ends
@@ -219,10 +223,15 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     if (ok) { atomicExch(&g_attn_status, 7); *s_abort = 1; }
     ok = false;
   };
-  int k = 0, sg = 0, row = row_of(u0), nt = first[row + 1] - first[row], head = (u0 - first[row] * kvh) / nt, t0 = u0 - first[row] * kvh - head * nt;
-  for (int u = u0; u < u1; ++sg) {                                     // tiles [t0, t1) of the nt tiles of (row, kv-head)
-    const int t1 = min(nt, t0 + (u1 - u));
-    u += t1 - t0;
+  int k = 0, sg = 0, row = row_of(u0), steps = first[row + 1] - first[row], head = (u0 - first[row] * kvh) / steps, at = u0 - first[row] * kvh - head * steps;
+  auto next_pair = [&]() {
+    at = 0;
+    if (++head == kvh) { head = 0; do ++row; while (row < P.rows && first[row + 1] == first[row]); steps = row < P.rows ? first[row + 1] - first[row] : 1; }
+  };
+  for (int u = u0; u < u1; ) {                                         // tiles [t0, t1) of the nt tiles of (row, kv-head)
+    const int to = min(steps, at + (u1 - u)), nt = steps - 1, t0 = max(0, at - 1), t1 = to - 1;
+    u += to - at;
+    if (t1 <= t0) { next_pair(); continue; }                           // the step without a tile, and this CTA's last
     const Place w = places[row];
     uint32_t qf[NT][HD / 16][2];
     wait(b_qfull + 8 * (sg & 1), sg >> 1);
@@ -375,8 +384,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
         }
       }
     compute_sync();                                                                         // the sums' places are free again
-    t0 = 0;
-    if (++head == kvh) { head = 0; do ++row; while (row < P.rows && first[row + 1] == first[row]); nt = row < P.rows ? first[row + 1] - first[row] : 1; }
+    ++sg;
+    next_pair();
   }
   if (P.beside) pdl_wait();
 }
@@ -473,9 +482,9 @@ template <int HD, int W> int launch_merge(const AttnP& P, bool bf, int slot_rows
 int ctas_of(int hd) { return SMS * (hd == 256 ? 1 : 2); }
 int slot_rows_of(int g) { return g <= 8 ? 8 : 16; }
 
-Work carve(void* ws, const yskn_paged_cache& c, int rows, int nh, int splits) {
+Work carve(void* ws, const yskn_paged_cache& c, int rows, int nh, size_t prefix_parts) {
   const int chunk = std::min(rows, ROWS), sr = slot_rows_of(nh / c.kvh);
-  const size_t pieces = (size_t)ctas_of(c.hd) + (size_t)chunk * c.kvh, parts = (size_t)rows * splits * nh;
+  const size_t pieces = (size_t)ctas_of(c.hd) + (size_t)chunk * c.kvh, parts = prefix_parts * nh;
   size_t at = 0;
   auto take = [&](size_t n) { const size_t x = at; at = (at + n + 255) / 256 * 256; return static_cast<uint8_t*>(ws) + x; };
   Work w;
@@ -518,14 +527,13 @@ int attn_status_fetch(int* out) {
 }  // namespace paged
 
 size_t paged_attention_bytes(const yskn_paged_cache& c, int rows, int nh, int shared) {
-  const int splits = shared > 0 ? paged_prefix_splits(rows, nh / c.kvh, c.kvh, shared) : 0;
-  return paged::carve(nullptr, c, rows, nh, splits).bytes;
+  return paged::carve(nullptr, c, rows, nh, shared > 0 ? paged_prefix_parts(rows, nh / c.kvh, c.kvh, shared) : 0).bytes;
 }
 
 int launch_paged_attention(const yskn_paged_cache& c, const yskn_paged_rows& r, const yskn_paged_attn_args& a, cudaStream_t st) {
   using namespace paged;
   const int g = a.nh / c.kvh, splits = a.shared > 0 ? paged_prefix_splits(r.rows, g, c.kvh, a.shared) : 0;
-  const Work w = carve(a.workspace, c, r.rows, a.nh, splits);
+  const Work w = carve(a.workspace, c, r.rows, a.nh, (size_t)r.rows * splits);
   if (splits > 0) if (int rc = launch_paged_prefix(c, r, a, splits, w, st)) return rc;
   for (int first = 0; first < r.rows; first += ROWS) {
     const int rows = std::min(ROWS, r.rows - first);

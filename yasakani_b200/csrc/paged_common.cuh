@@ -95,6 +95,7 @@ int launch_paged_attention(const yskn_paged_cache& c, const yskn_paged_rows& r, 
 size_t paged_attention_bytes(const yskn_paged_cache& c, int rows, int nh, int shared);
 size_t paged_select_bytes(const yskn_paged_cache& c, int rows, int blocks);
 int paged_prefix_splits(int rows, int g, int kvh, int shared);
+size_t paged_prefix_parts(int rows, int g, int kvh, int shared);
 int launch_paged_prefix(const yskn_paged_cache& c, const yskn_paged_rows& r, const yskn_paged_attn_args& a, int splits, const paged::Work& w, cudaStream_t st);
 
 namespace paged {

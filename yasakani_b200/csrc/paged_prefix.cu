@@ -434,16 +434,33 @@ int prefix_status_fetch(int* out) {
 
 }  // namespace paged
 
-// Runs of the prefix: as many as make the waves of CTA pairs shortest, a run's start and end counted as three tiles (Q in, O out).
+// Runs of the prefix for so many pairs of CTAs a kv-head: one wave of them where that goes, else what fills the waves best, a run's start and end counted as a
+// twentieth of a prefix.  It depends on the prefix only in that a run has a tile at least, so that a workspace for many rows and tokens serves fewer.
+static int prefix_runs(long long pairs, int kvh) {
+  const long long items = pairs * kvh, slots = paged::SMS / 2;
+  if (items <= slots) return (int)std::min<long long>(paged::MAX_SPLITS, slots / items);
+  int best = 1;
+  double cost = 0.0;
+  for (int s = 1; s <= 4; ++s) {
+    const double x = (double)((items * s + slots - 1) / slots) * (1.0 / s + 0.05);
+    if (s == 1 || x < cost) { cost = x; best = s; }
+  }
+  return best;
+}
+
 int paged_prefix_splits(int rows, int g, int kvh, int shared) {
   using namespace paged;
-  const long long items = (long long)pairs_of(rows, g) * kvh, slots = SMS / 2, nt = tiles_of(shared);
-  long long best = 1, cost = -1;
-  for (long long s = 1; s <= std::min<long long>(MAX_SPLITS, nt); ++s) {
-    const long long per = (nt + s - 1) / s, used = (nt + per - 1) / per, x = (items * used + slots - 1) / slots * (per + 3);
-    if (cost < 0 || x < cost) { cost = x; best = used; }
-  }
-  return (int)best;
+  const int nt = tiles_of(shared), s = std::min(prefix_runs(pairs_of(rows, g), kvh), nt), per = (nt + s - 1) / s;
+  return (nt + per - 1) / per;
+}
+
+// Partials (row, run) of any call with up to so many rows and shared tokens.
+size_t paged_prefix_parts(int rows, int g, int kvh, int shared) {
+  using namespace paged;
+  size_t most = 0;
+  const int tok = 128 / g, pairs = pairs_of(rows, g);
+  for (int p = 1; p <= pairs; ++p) most = std::max(most, (size_t)std::min<long long>(rows, 2ll * tok * p) * std::min(prefix_runs(p, kvh), tiles_of(shared)));
+  return most;
 }
 
 int launch_paged_prefix(const yskn_paged_cache& c, const yskn_paged_rows& r, const yskn_paged_attn_args& a, int splits, const paged::Work& w, cudaStream_t st) {
