@@ -104,24 +104,24 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
   pdl_launch();
 
   // ---- the line: first[r] = steps of one kv-head ahead of row r; a row's are one, without a tile, and its tiles.  Every warp finds it for itself (all write the same): no barrier between the positions and the first copy
+  int steps_of_all;
   {
     int below = 0;
-    for (int r0 = 0; r0 < ROWS; r0 += 32) {
+    for (int r0 = 0; r0 < P.rows; r0 += 32) {
       const int r = r0 + lane;
       int mine = 0;
       if (r < P.rows) { const Place w = place_of(P.R, r); places[r] = w; const int nt = tiles_of(P, w); mine = nt > 0 ? nt + 1 : 0; }
       int upto = mine;
-      if (r0 < P.rows) {
-        #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
-      }
+      #pragma unroll
+      for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
       first[r] = below + upto - mine;
       below += __shfl_sync(0xffffffffu, upto, 31);
     }
-    if (lane == 0) first[ROWS] = below;
+    if (lane == 0) first[P.rows] = below;
+    steps_of_all = below;
     __syncwarp();
   }
-  const int kvh = P.R.kvh, total = first[ROWS] * kvh, grid = min((int)gridDim.x, total), cta = (int)blockIdx.x;       // every CTA below `grid` has a step at least
+  const int kvh = P.R.kvh, total = steps_of_all * kvh, grid = min((int)gridDim.x, total), cta = (int)blockIdx.x;       // every CTA below `grid` has a step at least
   if (cta >= grid) { if (P.beside) pdl_wait(); return; }
   const int u0 = (int)((long long)total * cta / grid), u1 = (int)((long long)total * (cta + 1) / grid);
 
@@ -139,10 +139,13 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     // Boxes come 32 at a time, one a lane, looked up a batch ahead and across the borders of pairs: the lookups' latency (place, chosen block, table) is never
     // waited for.  A box: its row in the arrays, the position of its first token (no token: INT_MAX), its pair.
     struct Box { int at, base, pair; };
+    int base_row = row_of(u0);                                         // of the steps that are looked up: they lie a few rows on at most
     auto box_of = [&](int u, int j) {                                  // box j of step u; of a step without a tile: pair -1
       Box x{none, 0x7fffffff, -1};
       if (u >= u1) return x;
-      const int row = row_of(u), steps = first[row + 1] - first[row], in = u - first[row] * kvh, head = in / steps, t = in - head * steps - 1;
+      int row = base_row;
+      while (first[row + 1] * kvh <= u) ++row;
+      const int steps = first[row + 1] - first[row], in = u - first[row] * kvh, head = in / steps, t = in - head * steps - 1;
       if (t < 0) return x;
       const Place w = places[row];
       x.pair = row * kvh + head;
@@ -169,7 +172,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     Box now = box_of(u0 + tl, jl), next = now;
     for (int u = u0; u < u1 && ok; ++u) {
       int i = u - u0;
-      if (i > 0 && i % tpb == 0) now = next;
+      if (i > 0 && i % tpb == 0) { now = next; while (first[base_row + 1] * kvh <= u) ++base_row; }
       const bool look = i % tpb == min(3, tpb - 1);                    // for the next batch, once the ring is full
       const int behind = u - i % tpb + tpb + tl;
       i = (i % tpb) * npt + jl;
@@ -397,14 +400,15 @@ template <int HD, bool BF, int W>
 __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnP P, int slot_rows) {
   constexpr int V = HD / 128;                // float4 of a lane
   __shared__ float4 part[W > 1 ? W : 1][W > 1 ? HD / 4 : 1];
-  pdl_wait();
-  pdl_launch();
   const int lane = threadIdx.x & 31, wid = (int)(blockIdx.x * (MERGE_THREADS / 32) + (threadIdx.x >> 5)), x = wid / W, wi = wid % W;
   if (x >= P.rows * P.nh) return;            // the same for the whole block where W is its number of warps
   const int row = x / P.nh, head = x - row * P.nh, h = head / P.g, hh = head - h * P.g, pair = row * P.R.kvh + h;
-  const int2 span = P.span[pair];            // of a row without tiles nobody has written it, and nobody looks at it
+  // Ahead of the wait: the attention kernel lets this one start when all of its blocks have seen what lies in front of them finished, and writes no positions
   const Place w = place_of(P.R, row);
+  pdl_wait();
+  pdl_launch();
   if (w.seq < 0) return;
+  const int2 span = P.span[pair];            // of a row without tiles nobody has written it, and nobody looks at it
   const bool prefix = start_of(w, P.shared) > 0, own = tiles_of(P, w) > 0;
   if (!prefix && own && span.x == span.y) return;                      // finished where it was computed
   const int np = prefix ? P.splits : 0, n = np + (own ? span.y - span.x + 1 : 0);

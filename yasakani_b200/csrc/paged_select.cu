@@ -23,6 +23,7 @@ struct SelectP {
   const uint16_t* q; long long qs; const uint16_t* kmean;
   float2* approx; u64* exact;                // [row][kv-head][block]: score and sum of |q mean| (negative: no page); fp64 score as a sortable key, where it is needed
   int take; int* ids;
+  int scored;                                // the launch in front of the choice is the scores'
 };
 
 template <bool BF> __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -227,9 +228,13 @@ template <int HD, bool BF> __device__ u64 exact_key(const SelectP& P, const Plac
 template <int HD, bool BF>
 __global__ void __launch_bounds__(CT) paged_choose_kernel(const SelectP P) {
   __shared__ Shared sh;
+  const int row = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // Ahead of the wait, where the scores are: their kernel lets this one start when all of its blocks have seen what lies in front of them finished
+  Place w{-1, 0};
+  if (P.scored) w = place_of(P.R, row);
   pdl_wait();
   pdl_launch();
-  const int row = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (!P.scored) w = place_of(P.R, row);
   const size_t pair = (size_t)row * P.R.kvh + h;
   const float2* approx = P.approx + pair * P.R.blocks;
   u64* exact = P.exact + pair * P.R.blocks;
@@ -243,7 +248,6 @@ __global__ void __launch_bounds__(CT) paged_choose_kernel(const SelectP P) {
   read(0, P.R.blocks - 1);
   reinterpret_cast<int4*>(sh.hist)[tid] = make_int4(0, 0, 0, 0);
   if (tid == 0) sh.n = 0;
-  const Place w = place_of(P.R, row);
   if (w.seq < 0) return;
   const int last = w.vis > 0 ? (w.vis - 1) >> P.R.lp : -1, n = last > 0 ? last : 0;
   #pragma unroll
@@ -383,7 +387,7 @@ int launch_paged_select(const yskn_paged_cache& c, const yskn_paged_rows& r, con
   using namespace paged;
   const size_t n = (size_t)r.rows * c.kvh * r.blocks;
   SelectP P{rows_of(c, r, 0), r.rows, a.nh / c.kvh, a.nh, static_cast<const uint16_t*>(a.q), (long long)a.q_stride, static_cast<const uint16_t*>(c.kmean),
-            static_cast<float2*>(a.workspace), reinterpret_cast<u64*>(static_cast<float2*>(a.workspace) + n), a.take, a.ids};
+            static_cast<float2*>(a.workspace), reinterpret_cast<u64*>(static_cast<float2*>(a.workspace) + n), a.take, a.ids, r.blocks > 1 ? 1 : 0};
   const bool bf = c.dtype == YSKN_KV4_BF16;
   return c.hd == 256 ? (bf ? launch<256, true>(P, st) : launch<256, false>(P, st)) : (bf ? launch<128, true>(P, st) : launch<128, false>(P, st));
 }
