@@ -130,7 +130,7 @@ int yskn_kv4_paged_attention(const yskn_paged_cache* c, const yskn_paged_rows* r
   if (a->ids && a->shared > 0) KV4_REJECT("%s: chosen blocks and a shared part exclude one another", who);
   if (a->ids && (a->take <= 0 || (long long)a->take * c->page > 0x7fffffffll - 1024)) KV4_REJECT("%s: take %d", who, a->take);
   const long long tiles = (((a->ids ? (long long)a->take : (long long)r->blocks) * c->page) + TILE - 1) / TILE + 1;         // and a step without a tile
-  if (tiles * std::min(r->rows, 256) * c->kvh > 0x7fffffffll) KV4_REJECT("%s: %d rows of up to %lld tokens are too many for one call", who, r->rows, tiles * TILE);
+  if (tiles * std::min(r->rows, 224) * c->kvh > 0x7fffffffll) KV4_REJECT("%s: %d rows of up to %lld tokens are too many for one call", who, r->rows, tiles * TILE);
   const size_t need = paged_attention_bytes(*c, r->rows, a->nh, a->shared);
   if (!a->workspace || a->workspace_bytes < need) KV4_REJECT("%s: workspace of %zu bytes needed, %zu given", who, need, a->workspace ? a->workspace_bytes : (size_t)0);
   if ((uintptr_t)a->workspace & 255) KV4_REJECT("%s: the workspace must be 256-byte aligned", who);

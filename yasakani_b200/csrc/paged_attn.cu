@@ -30,7 +30,7 @@ __device__ int g_attn_status = 0;            // 0 ok; 7 = a bounded wait ran out
 
 namespace {
 
-constexpr int ROWS = 256;                    // rows of one launch
+constexpr int ROWS = 224;                    // rows of one launch (a multiple of 32; what shared memory leaves beside the ring)
 constexpr int NSLOT = 6;                     // half stages of the ring: K, V, K, V, K, V
 constexpr int CW = 4, NT_ = (CW + 1) * 32;   // compute warps; threads
 
@@ -45,9 +45,11 @@ struct AttnP {
 };
 
 template <int HD, int NT> struct Lay {
+  // Queries of pairs that have been asked for: of pairs of a tile or two their number is what the ring's depth is of long ones
+  static constexpr int NQ = NT == 1 ? 4 : 2;
   static constexpr int HALF = TILE * HD * 2, QP = HD * 2 + 16, PP = TILE * 2 + 16;   // bytes: a half stage; a row of Q; a row of P (paddings: eight rows on different banks)
-  static constexpr int OFF_Q = NSLOT * HALF, OFF_P = OFF_Q + 2 * NT * 8 * QP, OFF_MAX = OFF_P + 2 * NT * 8 * PP, OFF_L = OFF_MAX + 2 * CW * NT * 8 * 4;
-  static constexpr int OFF_BASE = OFF_L + CW * NT * 8 * 4, OFF_BAR = OFF_BASE + 3 * 4 * 4, OFF_PLACE = OFF_BAR + 16 * 8 + 8, OFF_FIRST = OFF_PLACE + ROWS * 8;
+  static constexpr int OFF_Q = NSLOT * HALF, OFF_P = OFF_Q + NQ * NT * 8 * QP, OFF_MAX = OFF_P + 2 * NT * 8 * PP, OFF_L = OFF_MAX + 2 * CW * NT * 8 * 4;
+  static constexpr int OFF_BASE = OFF_L + 2 * CW * NT * 8 * 4, OFF_BAR = OFF_BASE + 3 * 4 * 4, OFF_PLACE = OFF_BAR + 20 * 8 + 8, OFF_FIRST = OFF_PLACE + ROWS * 8;
   static constexpr int TOTAL = OFF_FIRST + (ROWS + 1) * 4;
   static constexpr int CTAS = HD == 256 ? 1 : 2;
   static_assert(HALF % 1024 == 0 && OFF_BASE % 16 == 0 && OFF_BAR % 8 == 0 && CTAS * (TOTAL + 1024) <= 228 * 1024, "shared memory");
@@ -85,13 +87,13 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sb = s_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t b_full = sb + L::OFF_BAR, b_empty = b_full + 8 * NSLOT, b_qfull = b_empty + 8 * NSLOT, b_qempty = b_qfull + 16;
-  volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::OFF_BAR + 16 * 8);
+  const uint32_t b_full = sb + L::OFF_BAR, b_empty = b_full + 8 * NSLOT, b_qfull = b_empty + 8 * NSLOT, b_qempty = b_qfull + 8 * L::NQ;
+  volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::OFF_BAR + 20 * 8);
   int* first = reinterpret_cast<int*>(smem + L::OFF_FIRST);
   Place* places = reinterpret_cast<Place*>(smem + L::OFF_PLACE);
   if (threadIdx.x == 0) {
     for (int i = 0; i < NSLOT; ++i) { bar_init(b_full + 8 * i, 1); bar_init(b_empty + 8 * i, CW); }
-    for (int i = 0; i < 2; ++i) { bar_init(b_qfull + 8 * i, 1); bar_init(b_qempty + 8 * i, CW); }
+    for (int i = 0; i < L::NQ; ++i) { bar_init(b_qfull + 8 * i, 1); bar_init(b_qempty + 8 * i, CW); }
     *s_abort = sb & 1023u ? 1 : 0;           // the swizzled tiles need a base of 1 KB
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&mapK) : "memory");
@@ -180,13 +182,13 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
       if (pr < 0) { if (look) next = box_of(behind, jl); continue; }
       if (pr != pair) {                                                // queries of the next pair
         pair = pr;
-        const int sg = queries;
-        if (sg >= 2 && !__all_sync(0xffffffffu, bar_wait(b_qempty + 8 * (sg & 1), ((sg >> 1) - 1) & 1))) { ok = false; break; }
-        if (lane == 0) bar_expect_tx(b_qfull + 8 * (sg & 1), P.g * HD * 2);
+        const int qb = queries % L::NQ;
+        if (queries >= L::NQ && !__all_sync(0xffffffffu, bar_wait(b_qempty + 8 * qb, (queries / L::NQ - 1) & 1))) { ok = false; break; }
+        if (lane == 0) bar_expect_tx(b_qfull + 8 * qb, P.g * HD * 2);
         __syncwarp();
         ++queries;
         const int row = pair / kvh, head = pair - row * kvh;
-        if (lane < P.g) bulk_1d(sb + L::OFF_Q + ((sg & 1) * NT * 8 + lane) * L::QP, P.q + row * P.qs + (size_t)(head * P.g + lane) * HD, HD * 2, b_qfull + 8 * (sg & 1));
+        if (lane < P.g) bulk_1d(sb + L::OFF_Q + (qb * NT * 8 + lane) * L::QP, P.q + row * P.qs + (size_t)(head * P.g + lane) * HD, HD * 2, b_qfull + 8 * qb);
       }
       #pragma unroll
       for (int v = 0; v < 2; ++v) {                                    // keys, values
@@ -208,7 +210,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     if (!ok) {                                                         // give up; the copies under way land before the block ends
       if (lane == 0) { atomicExch(&g_attn_status, 7); *s_abort = 1; }
       for (int it = max(0, issued - NSLOT); it < issued; ++it) bar_wait(b_full + 8 * (it % NSLOT), (it / NSLOT) & 1);
-      for (int it = max(0, queries - 2); it < queries; ++it) bar_wait(b_qfull + 8 * (it & 1), (it >> 1) & 1);
+      for (int it = max(0, queries - L::NQ); it < queries; ++it) bar_wait(b_qfull + 8 * (it % L::NQ), (it / L::NQ) & 1);
     }
     if (P.beside) pdl_wait();
     return;
@@ -237,17 +239,18 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     if (t1 <= t0) { next_pair(); continue; }                           // the step without a tile, and this CTA's last
     const Place w = places[row];
     uint32_t qf[NT][HD / 16][2];
-    wait(b_qfull + 8 * (sg & 1), sg >> 1);
+    const int qb = sg % L::NQ;
+    wait(b_qfull + 8 * qb, sg / L::NQ);
     #pragma unroll
     for (int n = 0; n < NT; ++n)
       #pragma unroll
       for (int i = 0; i < HD / 32; ++i) {
         uint32_t r[4];
-        ldm4(sb + L::OFF_Q + ((sg & 1) * NT * 8 + n * 8 + (lane & 7)) * L::QP + (4 * i + (lane >> 3)) * 16, r);
+        ldm4(sb + L::OFF_Q + (qb * NT * 8 + n * 8 + (lane & 7)) * L::QP + (4 * i + (lane >> 3)) * 16, r);
         qf[n][2 * i][0] = r[0]; qf[n][2 * i][1] = r[1]; qf[n][2 * i + 1][0] = r[2]; qf[n][2 * i + 1][1] = r[3];
       }
     __syncwarp();
-    if (lane == 0) bar_arrive(b_qempty + 8 * (sg & 1));
+    if (lane == 0) bar_arrive(b_qempty + 8 * qb);
 
     float o[NT][MT][4], m[NT][2], l[NT][2];
     #pragma unroll
@@ -355,7 +358,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
       for (int e = 0; e < 2; ++e) {
         #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
-        if (lane < 4) sl[warp * (NT * 8) + n * 8 + 2 * j + e] = l[n][e];
+        if (lane < 4) sl[((sg & 1) * CW + warp) * (NT * 8) + n * 8 + 2 * j + e] = l[n][e];
       }
     compute_sync();
     const bool direct = t1 - t0 == nt && start_of(w, P.shared) == 0;
@@ -369,7 +372,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
         const int h = n * 8 + 2 * j + e;
         float sum = 0.f;
         #pragma unroll
-        for (int i = 0; i < CW; ++i) sum += sl[i * (NT * 8) + h];
+        for (int i = 0; i < CW; ++i) sum += sl[((sg & 1) * CW + i) * (NT * 8) + h];
         if (h >= P.g || !ok) continue;
         if (direct) {
           uint16_t* dst = P.o16 + ((size_t)row * P.nh + head * P.g + h) * HD + warp * (HD / CW);
@@ -386,7 +389,6 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
           if (warp == 0 && g8 == 0) P.ml[piece * (NT * 8) + h] = make_float2(m[n][e], sum);
         }
       }
-    compute_sync();                                                                         // the sums' places are free again
     ++sg;
     next_pair();
   }

@@ -280,25 +280,26 @@ __global__ void __launch_bounds__(CT) paged_choose_kernel(const SelectP P) {
   const bool wild = !(e2 < (double)INFINITY), all = count <= P.take - 1;                     // all: no more candidates than places
 
   // ---- the bin that holds the border, and what may be on either side of it
-  double lo = -INFINITY, hi = INFINITY;                                 // scored in fp64: what is neither above hi nor below lo
+  float lo = -INFINITY, hi = INFINITY;                                  // scored in fp64: what is neither above hi nor below lo (rounded outwards)
   if (!wild && !all) {
     const float flo = float_of(klo), fhi = float_of(khi), scale = (float)BINS / (fhi - flo);
-    lo = (double)flo - e2; hi = (double)fhi + e2;
+    lo = __double2float_rd((double)flo - e2); hi = __double2float_ru((double)fhi + e2);
     if (fhi - flo < INFINITY && scale < INFINITY) {                     // else all are unsure: scores that are as good as equal, or a range beyond fp32
       each([&](int, const float2& f) { if (f.y >= 0.f) atomicAdd(&sh.hist[min(BINS - 1, (int)((f.x - flo) * scale))], 1); });
       int left = P.take - 1;
       const double bin = (double)border_bin(sh, left), step = 1.0 / (double)scale;
       // a score's bin is rounded by less than 2^-9 of a bin
-      lo = fmax((double)flo, (double)flo + (bin - 0.01) * step) - e2; hi = fmin((double)fhi, (double)flo + (bin + 1.01) * step) + e2;
+      lo = __double2float_rd(fmax((double)flo, (double)flo + (bin - 0.01) * step) - e2);
+      hi = __double2float_ru(fmin((double)fhi, (double)flo + (bin + 1.01) * step) + e2);
     }
   }
-  auto unsure = [&](const float2& f) { return f.y >= 0.f && !((double)f.x > hi) && !((double)f.x < lo); };
+  auto unsure = [&](const float2& f) { return f.y >= 0.f && !(f.x > hi) && !(f.x < lo); };
   // ---- the unsure ones: how many, which
   int sure = 0, many = 0;
   if (!all) {
     each([&](int i, const float2& f) {
       if (unsure(f)) { const int at = atomicAdd(&sh.n, 1); if (at < LIST) sh.at[at] = i; }
-      else if (f.y >= 0.f && (double)f.x > hi) ++sure;
+      else if (f.y >= 0.f && f.x > hi) ++sure;
     });
     sure = __reduce_add_sync(ALL, sure);
     if (lane == 0) sh.warps[warp] = sure;
@@ -340,7 +341,7 @@ __global__ void __launch_bounds__(CT) paged_choose_kernel(const SelectP P) {
       const float2 f = x[e];
       what[e] = 0;
       if (f.y >= 0.f) {
-        if (all || (double)f.x > hi) what[e] = 1;
+        if (all || f.x > hi) what[e] = 1;
         else if (unsure(f)) {
           if (!need) what[e] = 1;
           else if (listed) what[e] = (sh.hist[i >> 5] >> (i & 31)) & 1;
