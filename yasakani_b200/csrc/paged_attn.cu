@@ -127,12 +127,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
   if (cta >= grid) { if (P.beside) pdl_wait(); return; }
   const int u0 = (int)((long long)total * cta / grid), u1 = (int)((long long)total * (cta + 1) / grid);
 
-  // The row that holds step u: the last whose first step is not behind it
-  auto row_of = [&](int u) {
-    int lo = 0, hi = P.rows - 1;
-    while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (first[mid] * kvh <= u) lo = mid; else hi = mid - 1; }
-    return lo;
-  };
+  int row = 0;                               // the row that holds step u0: the last whose first step is not behind it
+  for (int hi = P.rows - 1; row < hi; ) { const int mid = (row + hi + 1) >> 1; if (first[mid] * kvh <= u0) row = mid; else hi = mid - 1; }
   const int lc = min(P.R.lp, 6), chunk = 1 << lc, npt = TILE >> lc;    // rows of a box, boxes of a tile
 
   if (warp == CW) {
@@ -141,11 +137,12 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     // Boxes come 32 at a time, one a lane, looked up a batch ahead and across the borders of pairs: the lookups' latency (place, chosen block, table) is never
     // waited for.  A box: its row in the arrays, the position of its first token (no token: INT_MAX), its pair.
     struct Box { int at, base, pair; };
-    int base_row = row_of(u0);                                         // of the steps that are looked up: they lie a few rows on at most
+    int base_row = row;                                                // of the steps that are looked up: they lie a few rows on at most
     auto box_of = [&](int u, int j) {                                  // box j of step u; of a step without a tile: pair -1
       Box x{none, 0x7fffffff, -1};
       if (u >= u1) return x;
       int row = base_row;
+      #pragma unroll 1
       while (first[row + 1] * kvh <= u) ++row;
       const int steps = first[row + 1] - first[row], in = u - first[row] * kvh, head = in / steps, t = in - head * steps - 1;
       if (t < 0) return x;
@@ -171,15 +168,18 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     int k = 0, pair = -1, issued = 0, queries = 0;                     // tiles so far; the pair they belong to; half stages and queries asked for
     bool ok = *s_abort == 0;
     const int tpb = 32 / npt, jl = lane & (npt - 1), tl = lane / npt;  // tiles of a batch; this lane's box and tile in it
-    Box now = box_of(u0 + tl, jl), next = now;
+    Box now{}, next{};
     for (int u = u0; u < u1 && ok; ++u) {
       int i = u - u0;
-      if (i > 0 && i % tpb == 0) { now = next; while (first[base_row + 1] * kvh <= u) ++base_row; }
-      const bool look = i % tpb == min(3, tpb - 1);                    // for the next batch, once the ring is full
-      const int behind = u - i % tpb + tpb + tl;
-      i = (i % tpb) * npt + jl;
+      const int in = i % tpb;
+      if (i == 0 || in == 4) {                                         // the first batch; the one behind this, once the ring is full (in one place: every line of cold code counts)
+        const Box x = box_of(i == 0 ? u0 + tl : u - in + tpb + tl, jl);
+        if (i == 0) now = x; else next = x;
+      }
+      if (i > 0 && in == 0) { now = next; while (first[base_row + 1] * kvh <= u) ++base_row; }
+      i = in * npt + jl;
       const int at = __shfl_sync(0xffffffffu, now.at, i), base = __shfl_sync(0xffffffffu, now.base, i), pr = __shfl_sync(0xffffffffu, now.pair, i);
-      if (pr < 0) { if (look) next = box_of(behind, jl); continue; }
+      if (pr < 0) continue;
       if (pr != pair) {                                                // queries of the next pair
         pair = pr;
         const int qb = queries % L::NQ;
@@ -205,7 +205,6 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
         if (lane < npt) tma_3d(sb + slot * L::HALF + lane * (chunk * HD * 2), v ? &mapV : &mapK, 0, at, 0, b_full + 8 * slot);
       }
       ++k;
-      if (look) next = box_of(behind, jl);
     }
     if (!ok) {                                                         // give up; the copies under way land before the block ends
       if (lane == 0) { atomicExch(&g_attn_status, 7); *s_abort = 1; }
@@ -228,15 +227,11 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     if (ok) { atomicExch(&g_attn_status, 7); *s_abort = 1; }
     ok = false;
   };
-  int k = 0, sg = 0, row = row_of(u0), steps = first[row + 1] - first[row], head = (u0 - first[row] * kvh) / steps, at = u0 - first[row] * kvh - head * steps;
-  auto next_pair = [&]() {
-    at = 0;
-    if (++head == kvh) { head = 0; do ++row; while (row < P.rows && first[row + 1] == first[row]); steps = row < P.rows ? first[row + 1] - first[row] : 1; }
-  };
-  for (int u = u0; u < u1; ) {                                         // tiles [t0, t1) of the nt tiles of (row, kv-head)
+  int k = 0, sg = 0, steps = first[row + 1] - first[row], head = (u0 - first[row] * kvh) / steps, at = u0 - first[row] * kvh - head * steps;
+  for (int u = u0; ; ) {                                               // tiles [t0, t1) of the nt tiles of (row, kv-head)
     const int to = min(steps, at + (u1 - u)), nt = steps - 1, t0 = max(0, at - 1), t1 = to - 1;
     u += to - at;
-    if (t1 <= t0) { next_pair(); continue; }                           // the step without a tile, and this CTA's last
+    if (t1 > t0) {                                                     // else the step without a tile, and this CTA's last
     const Place w = places[row];
     uint32_t qf[NT][HD / 16][2];
     const int qb = sg % L::NQ;
@@ -390,7 +385,10 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
         }
       }
     ++sg;
-    next_pair();
+    }
+    if (u >= u1) break;
+    at = 0;                                                            // the next pair
+    if (++head == kvh) { head = 0; do ++row; while (row < P.rows && first[row + 1] == first[row]); steps = row < P.rows ? first[row + 1] - first[row] : 1; }
   }
   if (P.beside) pdl_wait();
 }
