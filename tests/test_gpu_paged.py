@@ -283,6 +283,30 @@ def test_choice_of_blocks(dt, nh, hkv, hd, page, lengths, take):
     assert torch.equal(ids.cpu(), want)
 
 
+@pytest.mark.parametrize("blocks,take,kind", [(5000, 33, "random"), (9001, 1024, "random"), (4097, 300, "equal"), (6000, 50, "few values"), (70000, 20, "few values"),
+                                              (66000, 100, "random"), (5000, 40, "not finite")])
+def test_choice_among_many_blocks(blocks, take, kind):
+    """More blocks than a thread block keeps in registers, or has bits for; scores that are equal, or that fp32 cannot tell apart, or does not hold."""
+    from yasakani_b200 import paged
+    g = torch.Generator(device="cuda").manual_seed(blocks)
+    k = torch.zeros((blocks, 1, 16, 128), dtype=torch.bfloat16, device="cuda")
+    kmean = torch.randn((blocks, 1, 128), generator=g, device="cuda").bfloat16()
+    if kind == "equal":
+        kmean[:] = kmean[0]
+    if kind == "few values":
+        kmean = kmean[torch.randint(0, 40, (blocks,), generator=g, device="cuda")].contiguous()
+    if kind == "not finite":
+        kmean[torch.randint(0, blocks, (500,), generator=g, device="cuda"), 0, 5] = float("inf")
+        kmean[77, 0, 3] = float("nan")
+        kmean[78, 0] = 3e38
+    table = torch.randperm(blocks, generator=g, device="cuda").to(torch.int32)[None].contiguous()
+    q = torch.randn((1, 3, 128), generator=g, device="cuda").bfloat16()
+    cache = paged.PagedCache.of(k, k, kmean)
+    ids = torch.full((1, 1, take), 99, dtype=torch.int32, device="cuda")
+    paged.launch_select(q, cache, table, ints([0]), ints([blocks * 16 - 1]), ids, paged.workspace(cache, 1, 3, blocks, select=True))
+    assert torch.equal(ids.cpu(), choose(q, kmean, table, [0], [blocks * 16 - 1], 16, take))
+
+
 def test_choice_among_equal_scores_takes_the_lowest_blocks():
     from yasakani_b200 import paged
     k, v, table, g = make_pool([64 * 600], 2, 128, 64, torch.float16, seed=1)

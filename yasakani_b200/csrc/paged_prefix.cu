@@ -420,6 +420,7 @@ int launch(const yskn_paged_cache& c, const PrefixP& P, int pairs, cudaStream_t 
   return launch_pdl("paged_prefix_kernel", kern, dim3(2u * pairs, (unsigned)P.splits, (unsigned)c.kvh), THREADS, L::TOTAL, st, mk, mv, P);
 }
 
+int most_runs(int tiles) { return (tiles + 1) / 2; }
 int pairs_of(int rows, int g) { const int tok = 128 / g; return (rows + 2 * tok - 1) / (2 * tok); }
 
 }  // namespace
@@ -435,7 +436,8 @@ int prefix_status_fetch(int* out) {
 }  // namespace paged
 
 // Runs of the prefix for so many pairs of CTAs a kv-head: one wave of them where that goes, else what fills the waves best, a run's start and end counted as a
-// twentieth of a prefix.  It depends on the prefix only in that a run has a tile at least, so that a workspace for many rows and tokens serves fewer.
+// twentieth of a prefix.  It depends on the prefix only in that a run has two tiles at least (one: a short prefix takes the SMs from the rows' own part beside it, 8 rows
+// behind 4,096 tokens 14.9 us, with two 12.3, three 13.2, four 14.0), so that a workspace for many rows and tokens serves fewer.
 static int prefix_runs(long long pairs, int kvh) {
   const long long items = pairs * kvh, slots = paged::SMS / 2;
   if (items <= slots) return (int)std::min<long long>(paged::MAX_SPLITS, slots / items);
@@ -450,7 +452,7 @@ static int prefix_runs(long long pairs, int kvh) {
 
 int paged_prefix_splits(int rows, int g, int kvh, int shared) {
   using namespace paged;
-  const int nt = tiles_of(shared), s = std::min(prefix_runs(pairs_of(rows, g), kvh), nt), per = (nt + s - 1) / s;
+  const int nt = tiles_of(shared), s = std::min(prefix_runs(pairs_of(rows, g), kvh), most_runs(nt)), per = (nt + s - 1) / s;
   return (nt + per - 1) / per;
 }
 
@@ -459,7 +461,7 @@ size_t paged_prefix_parts(int rows, int g, int kvh, int shared) {
   using namespace paged;
   size_t most = 0;
   const int tok = 128 / g, pairs = pairs_of(rows, g);
-  for (int p = 1; p <= pairs; ++p) most = std::max(most, (size_t)std::min<long long>(rows, 2ll * tok * p) * std::min(prefix_runs(p, kvh), tiles_of(shared)));
+  for (int p = 1; p <= pairs; ++p) most = std::max(most, (size_t)std::min<long long>(rows, 2ll * tok * p) * std::min(prefix_runs(p, kvh), most_runs(tiles_of(shared))));
   return most;
 }
 

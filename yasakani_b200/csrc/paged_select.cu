@@ -294,18 +294,39 @@ __global__ void __launch_bounds__(CT) paged_choose_kernel(const SelectP P) {
     }
   }
   auto unsure = [&](const float2& f) { return f.y >= 0.f && !(f.x > hi) && !(f.x < lo); };
-  // ---- the unsure ones: how many, which
+  // ---- how many are chosen for sure, how many are unsure, and which those are
   int sure = 0, many = 0;
   if (!all) {
+    int mine = 0;                                                       // sure ones, and unsure ones << 16
     each([&](int i, const float2& f) {
-      if (unsure(f)) { const int at = atomicAdd(&sh.n, 1); if (at < LIST) sh.at[at] = i; }
-      else if (f.y >= 0.f && f.x > hi) ++sure;
+      if (unsure(f)) { const int at = atomicAdd(&sh.n, 1); if (at < LIST) sh.at[at] = i; mine += 1 << 16; }
+      else if (f.y >= 0.f && f.x > hi) ++mine;
     });
-    sure = __reduce_add_sync(ALL, sure);
-    if (lane == 0) sh.warps[warp] = sure;
-    __syncthreads();
-    sure = of_all(sh, lane);
-    many = sh.n;
+    if (n <= PER * CT) {                                                // one walk: places are known with the counts
+      const int upto = upto_lane(mine, lane);
+      if (lane == 31) sh.warps[warp] = upto;
+      __syncthreads();
+      const int before = ahead_of(sh, warp, lane) + upto - mine;
+      const int total = of_all(sh, lane);
+      sure = total & 0xffff; many = total >> 16;
+      if (many <= P.take - 1 - sure) {                                  // the unsure ones are all chosen, as mostly: the border itself and nothing else
+        int at = (before & 0xffff) + (before >> 16);
+        #pragma unroll
+        for (int e = 0; e < PER; ++e) if (x[e].y >= 0.f && !(x[e].x < lo)) ids[at++] = PER * tid + e;
+        if (tid == 0) ids[sure + many] = last;
+        for (int i = sure + many + 1 + tid; i < P.take; i += CT) ids[i] = -1;
+        return;
+      }
+    } else {
+      // 16 bits do not hold more: counted on their own
+      int s2 = 0;
+      each([&](int, const float2& f) { if (f.y >= 0.f && f.x > hi && !unsure(f)) ++s2; });
+      s2 = __reduce_add_sync(ALL, s2);
+      if (lane == 0) sh.warps[warp] = s2;
+      __syncthreads();
+      sure = of_all(sh, lane);
+      many = sh.n;
+    }
   }
   int left = P.take - 1 - sure;                                         // places for the unsure ones
   u64 cut = 0;                                                          // of these: above `cut`, and the first `left` equal to it
@@ -353,8 +374,8 @@ __global__ void __launch_bounds__(CT) paged_choose_kernel(const SelectP P) {
     const int upto = upto_lane(mine, lane);
     if (lane == 31) sh.warps[warp] = upto;
     __syncthreads();
-    const int before = ahead_of(sh, warp, lane) + upto - mine, total = of_all(sh, lane);
-    int a = before & 0xffff, e0 = equal + (before >> 16);
+    const int ahead = ahead_of(sh, warp, lane) + upto - mine, total = of_all(sh, lane);
+    int a = ahead & 0xffff, e0 = equal + (ahead >> 16);
     #pragma unroll
     for (int e = 0; e < PER; ++e) {
       if (what[e] == 1 || (what[e] > 1 && e0 < left)) ids[at + a + min(e0, left) - min(equal, left)] = i0 + PER * tid + e;
