@@ -32,21 +32,21 @@ struct AppendP {
 
 constexpr int SLOTS = 4;                     // 16-byte loads a lane has in flight: 4 KB a warp
 
-// Two channels' worth of a 32-bit word, a, turned with the other channels of their pairs, d: first half of the rotated channels a cos - d sin, second half a cos + d sin.
-template <bool BF> __device__ __forceinline__ uint32_t turn(uint32_t aw, uint32_t dw, float c0, float s0, float c1, float s1, bool lower) {
+// Two channels' worth of a 32-bit word, a, turned with the other channels of their pairs, d: a cos + d sin, the sine's sign being that of the channel's half.
+template <bool BF> __device__ __forceinline__ uint32_t turn(uint32_t aw, uint32_t dw, const float4& t) {
   const float2 a = unpack16<BF>(aw), d = unpack16<BF>(dw);
-  return pack16<BF>(fmaf(d.x, lower ? -s0 : s0, a.x * c0), fmaf(d.y, lower ? -s1 : s1, a.y * c1));
+  return pack16<BF>(fmaf(d.x, t.y, a.x * t.x), fmaf(d.y, t.w, a.y * t.z));
 }
-template <bool BF> __device__ __forceinline__ uint4 turn8(const uint4& a, const uint4& d, const float4 (&t)[4], bool lower) {
-  return make_uint4(turn<BF>(a.x, d.x, t[0].x, t[0].y, t[0].z, t[0].w, lower), turn<BF>(a.y, d.y, t[1].x, t[1].y, t[1].z, t[1].w, lower),
-                    turn<BF>(a.z, d.z, t[2].x, t[2].y, t[2].z, t[2].w, lower), turn<BF>(a.w, d.w, t[3].x, t[3].y, t[3].z, t[3].w, lower));
+template <bool BF> __device__ __forceinline__ uint4 turn8(const uint4& a, const uint4& d, const float4 (&t)[4]) {
+  return make_uint4(turn<BF>(a.x, d.x, t[0]), turn<BF>(a.y, d.y, t[1]), turn<BF>(a.z, d.z, t[2]), turn<BF>(a.w, d.w, t[3]));
 }
-// (cos, sin) of channels ch .. ch + 7 at a position; ch < rd.
+// (cos, sin) of channels ch .. ch + 7 at a position, ch < rd; -sin in the first half of the rotated channels.
 __device__ __forceinline__ void angles(const AppendP& P, int pos, int ch, float4 (&t)[4]) {
   const int half = P.rd / 2;
-  const float4* src = reinterpret_cast<const float4*>(P.rope + ((size_t)pos * half + (ch < half ? ch : ch - half)) * 2);
+  const bool lower = ch < half;
+  const float4* src = reinterpret_cast<const float4*>(P.rope + ((size_t)pos * half + (lower ? ch : ch - half)) * 2);
   #pragma unroll
-  for (int e = 0; e < 4; ++e) t[e] = src[e];
+  for (int e = 0; e < 4; ++e) { const float4 f = src[e]; t[e] = lower ? make_float4(f.x, -f.y, f.z, -f.w) : f; }
 }
 // The page of a row, -1 where the row is left out; `at` its position.
 __device__ __forceinline__ int page_of_row(const AppendP& P, int row, int& at) {
@@ -100,7 +100,7 @@ __device__ void page_means(const AppendP& P, int r0, int h) {
         if (ch < P.rd) {
           float4 cs[4];
           angles(P, first + t, ch, cs);
-          u = turn8<BF>(u, *reinterpret_cast<const uint4*>(src + (ch < half ? ch + half : ch - half)), cs, ch < half);
+          u = turn8<BF>(u, *reinterpret_cast<const uint4*>(src + (ch < half ? ch + half : ch - half)), cs);
         }
       }
       const uint32_t u4[4] = {u.x, u.y, u.z, u.w};
@@ -156,25 +156,26 @@ __global__ void __launch_bounds__(256, 4) paged_append_kernel(const AppendP P) {
   float4 cs[4];
   if (ch < P.rd) angles(P, pos, ch, cs);
   const int partner = ch < half ? lane + lh : ch < P.rd ? lane - lh : lane;
+  uint16_t* const q_row = P.q_out + (size_t)row * P.nh * HD + ch;
+  const size_t place = (((size_t)page * kvh) << P.R.lp) + (pos & (P.R.page - 1));            // of kv-head 0; the others a page's rows further each
   #pragma unroll
   for (int i = 0; i < SLOTS; ++i) {
+    const int h = vh[i];
     uint4 y = x[i];
-    if (P.rd > 0) {
+    if (P.rd > 0 && (s0 + i) * (256 / HD) < nq + kvh) {                // not a slot of values alone: the same for the whole warp
       uint4 o;
       o.x = __shfl_sync(0xffffffffu, y.x, partner); o.y = __shfl_sync(0xffffffffu, y.y, partner);
       o.z = __shfl_sync(0xffffffffu, y.z, partner); o.w = __shfl_sync(0xffffffffu, y.w, partner);
-      if (ch < P.rd && vh[i] < nq + kvh) y = turn8<BF>(y, o, cs, ch < half);
+      if (ch < P.rd && h < nq + kvh) y = turn8<BF>(y, o, cs);
     }
-    if (vh[i] < 0) continue;
+    if (h < 0 || (h >= nq && page < 0)) continue;
     uint16_t* dst;
-    if (vh[i] < nq) dst = P.q_out + ((size_t)row * P.nh + vh[i]) * HD;
+    if (h < nq) dst = q_row + h * HD;
     else {
-      if (page < 0) continue;
-      const int h = vh[i] - nq;
-      const size_t at = (((size_t)page * kvh + (h < kvh ? h : h - kvh)) << P.R.lp) + (pos & (P.R.page - 1));
-      dst = (h < kvh ? P.k : P.v) + at * HD;
+      const int j = h - nq, jj = j < kvh ? j : j - kvh;
+      dst = (j < kvh ? P.k : P.v) + (place + ((size_t)jj << P.R.lp)) * HD + ch;
     }
-    __stcs(reinterpret_cast<uint4*>(dst + ch), y);
+    __stcs(reinterpret_cast<uint4*>(dst), y);
   }
 }
 
