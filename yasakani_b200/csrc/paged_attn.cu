@@ -393,14 +393,14 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
   if (P.beside) pdl_wait();
 }
 
-// Joins what the parts of a (row, head) hold: partials over the shared prefix, then pieces of CTAs.  W warps a (row, head): each looks at all parts' maxima and sums by itself,
-// a lane a part, and adds up every W-th part's O, HD / 32 channels a lane.
+// Joins what the parts of a (row, head) hold: partials over the shared prefix, then pieces of CTAs.  W warps for 128 channels of a (row, head), four a lane: each looks at all
+// parts' maxima and sums by itself, a lane a part, and adds up every W-th part's O, U of them asked for together.
 constexpr int MERGE_THREADS = 256;
-template <int HD, bool BF, int W>
+template <int HD, bool BF, int W, int U>
 __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnP P, int slot_rows) {
-  constexpr int V = HD / 128;                // float4 of a lane
-  __shared__ float4 part[W > 1 ? W : 1][W > 1 ? HD / 4 : 1];
-  const int lane = threadIdx.x & 31, wid = (int)(blockIdx.x * (MERGE_THREADS / 32) + (threadIdx.x >> 5)), x = wid / W, wi = wid % W;
+  constexpr int V = HD / 128;
+  __shared__ float4 part[W][W > 1 ? 32 : 1];
+  const int lane = threadIdx.x & 31, wid = (int)(blockIdx.x * (MERGE_THREADS / 32) + (threadIdx.x >> 5)), xv = wid / W, x = xv / V, v = xv % V, wi = wid % W;
   if (x >= P.rows * P.nh) return;            // the same for the whole block where W is its number of warps
   const int row = x / P.nh, head = x - row * P.nh, h = head / P.g, hh = head - h * P.g, pair = row * P.R.kvh + h;
   // Ahead of the wait: the attention kernel lets this one start when all of its blocks have seen what lies in front of them finished, and writes no positions
@@ -413,22 +413,18 @@ __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnP 
   if (!prefix && own && span.x == span.y) return;                      // finished where it was computed
   const int np = prefix ? P.splits : 0, n = np + (own ? span.y - span.x + 1 : 0);
   const float2* qml = P.qml + (size_t)row * P.splits * P.nh + head;
-  const float* qacc = P.qacc + ((size_t)row * P.splits * P.nh + head) * HD;
+  const float* qacc = P.qacc + ((size_t)row * P.splits * P.nh + head) * HD + 128 * v;
   const size_t piece0 = ((size_t)span.x + pair) * slot_rows + hh;      // piece c of the pair: + c * slot_rows
   auto ml_at = [&](int i) { return i < np ? qml[(size_t)i * P.nh] : P.ml[piece0 + (size_t)(i - np) * slot_rows]; };
-  auto o_at = [&](int i) { return i < np ? qacc + (size_t)i * P.nh * HD : P.pacc + (piece0 + (size_t)(i - np) * slot_rows) * HD; };
-  constexpr int U = W > 1 ? 8 : 4, PC = U * W;           // parts that a warp asks for together; parts of all W warps
+  auto o_at = [&](int i) { return i < np ? qacc + (size_t)i * P.nh * HD : P.pacc + (piece0 + (size_t)(i - np) * slot_rows) * HD + 128 * v; };
+  constexpr int PC = U * W;                  // parts that all W warps ask for together
   auto ml_or = [&](int i) { return i < n ? ml_at(i) : make_float2(-INFINITY, 0.f); };
-  float4 o[U][V];
+  float4 o[U];
   auto ask = [&](int c) {                    // O of this warp's parts c + wi + W u: beside the maxima and sums, not behind them
     #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = c + wi + W * u;
-      if (i < n) {
-        const float4* src = reinterpret_cast<const float4*>(o_at(i)) + lane;
-        #pragma unroll
-        for (int v = 0; v < V; ++v) o[u][v] = src[32 * v];
-      }
+      if (i < n) o[u] = reinterpret_cast<const float4*>(o_at(i))[lane];
     }
   };
   float2 f0 = ml_or(lane), f1 = ml_or(32 + lane);
@@ -439,9 +435,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnP 
   for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   if (top == -INFINITY) top = 0.f;
   float sum = 0.f;
-  float4 acc[V];
-  #pragma unroll
-  for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int c = 0; c < n; c += PC) {
     if (c > 0) { f0 = ml_or(c + lane); f1 = PC > 32 ? ml_or(c + 32 + lane) : f1; ask(c); }
     const float w0 = lane < PC && f0.y != 0.f ? ex2(f0.x - top) : 0.f, w1 = PC > 32 && f1.y != 0.f ? ex2(f1.x - top) : 0.f;
@@ -450,36 +444,28 @@ __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnP 
     #pragma unroll
     for (int u = 0; u < U; ++u) {
       const float wk = __shfl_sync(0xffffffffu, W * u < 32 ? w0 : w1, (wi + W * u) & 31);
-      if (wk != 0.f) {                       // a part without weight may hold anything
-        #pragma unroll
-        for (int v = 0; v < V; ++v) { acc[v].x += wk * o[u][v].x; acc[v].y += wk * o[u][v].y; acc[v].z += wk * o[u][v].z; acc[v].w += wk * o[u][v].w; }
-      }
+      if (wk != 0.f) { acc.x += wk * o[u].x; acc.y += wk * o[u].y; acc.z += wk * o[u].z; acc.w += wk * o[u].w; }      // a part without weight may hold anything
     }
   }
   #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   if (W > 1) {
-    #pragma unroll
-    for (int v = 0; v < V; ++v) part[W > 1 ? wi : 0][W > 1 ? 32 * v + lane : 0] = acc[v];
+    part[wi][W > 1 ? lane : 0] = acc;
     __syncthreads();
-    if (wi >= V) return;                     // warp v finishes channels 128 v .. 128 v + 127
-    acc[0] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (wi > 0) return;
     #pragma unroll
-    for (int i = 0; i < W; ++i) { const float4 f = part[W > 1 ? i : 0][W > 1 ? 32 * wi + lane : 0]; acc[0].x += f.x; acc[0].y += f.y; acc[0].z += f.z; acc[0].w += f.w; }
+    for (int i = 1; i < W; ++i) { const float4 f = part[i][W > 1 ? lane : 0]; acc.x += f.x; acc.y += f.y; acc.z += f.z; acc.w += f.w; }
   }
   const float inv = 1.f / sum;
-  #pragma unroll
-  for (int v = 0; v < (W > 1 ? 1 : V); ++v) {
-    uint2 y;
-    y.x = sum == 0.f ? 0u : pack16<BF>(acc[v].x * inv, acc[v].y * inv);
-    y.y = sum == 0.f ? 0u : pack16<BF>(acc[v].z * inv, acc[v].w * inv);
-    *reinterpret_cast<uint2*>(P.o16 + (size_t)x * HD + 4 * (32 * (W > 1 ? wi : v) + lane)) = y;
-  }
+  uint2 y;
+  y.x = sum == 0.f ? 0u : pack16<BF>(acc.x * inv, acc.y * inv);
+  y.y = sum == 0.f ? 0u : pack16<BF>(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(P.o16 + (size_t)x * HD + 128 * v + 4 * lane) = y;
 }
 
-template <int HD, int W> int launch_merge(const AttnP& P, bool bf, int slot_rows, cudaStream_t st) {
-  auto kern = bf ? paged_merge_kernel<HD, true, W> : paged_merge_kernel<HD, false, W>;
-  const long long warps = (long long)P.rows * P.nh * W;
+template <int HD, int W, int U> int launch_merge(const AttnP& P, bool bf, int slot_rows, cudaStream_t st) {
+  auto kern = bf ? paged_merge_kernel<HD, true, W, U> : paged_merge_kernel<HD, false, W, U>;
+  const long long warps = (long long)P.rows * P.nh * (HD / 128) * W;
   return launch_pdl("paged_merge_kernel", kern, dim3((unsigned)((warps + 7) / 8)), MERGE_THREADS, 0, st, P, slot_rows);
 }
 
@@ -546,11 +532,14 @@ int launch_paged_attention(const yskn_paged_cache& c, const yskn_paged_rows& r, 
             static_cast<uint16_t*>(a.o16) + (size_t)first * a.nh * c.hd, splits > 0 ? a.shared : 0, a.ids ? a.ids + (size_t)first * c.kvh * a.take : nullptr, a.take,
             w.span, w.ml, w.pacc, w.qml + part, w.qacc + part * c.hd, splits, splits > 0 && first == 0 ? 1 : 0};
     if (int rc = c.hd == 256 ? dispatch<256>(c, P, st) : dispatch<128>(c, P, st)) return rc;
-    // few rows: their parts are many, a block adds them up together; many rows: few parts each, a warp does
-    const bool bf = c.dtype == YSKN_KV4_BF16, few = (long long)rows * a.nh <= 2 * SMS;
-    const int sr = slot_rows_of(g);
-    const int rc = c.hd == 256 ? (few ? launch_merge<256, 8>(P, bf, sr, st) : launch_merge<256, 1>(P, bf, sr, st))
-                               : (few ? launch_merge<128, 8>(P, bf, sr, st) : launch_merge<128, 1>(P, bf, sr, st));
+    // Few rows have many parts: eight warps each.  More have few: a warp, which asks for eight parts at once where there are SMs for all of them (16 rows of 28 heads over
+    // 33 blocks with their choice 33.6 us, four at once 34.7), and for four where its registers count (200 rows of 28 heads behind 5,216 tokens 62.4 us, eight 63.7)
+    const bool bf = c.dtype == YSKN_KV4_BF16;
+    const long long items = (long long)rows * a.nh;
+    const int sr = slot_rows_of(g), rc =
+        items <= 2 * SMS ? (c.hd == 256 ? launch_merge<256, 8, 8>(P, bf, sr, st) : launch_merge<128, 8, 8>(P, bf, sr, st))
+        : items * (c.hd / 128) <= 8 * SMS ? (c.hd == 256 ? launch_merge<256, 1, 8>(P, bf, sr, st) : launch_merge<128, 1, 8>(P, bf, sr, st))
+                                          : (c.hd == 256 ? launch_merge<256, 1, 4>(P, bf, sr, st) : launch_merge<128, 1, 4>(P, bf, sr, st));
     if (rc) return rc;
   }
   return 0;
