@@ -82,10 +82,11 @@ YSKN_KV4_API const char* yskn_kv4_build_info(void);   /* yskn_build_info, src/c_
  * rejected).  Process-wide; the counterpart of the reference's YSKN_ATTN_GENERIC switch (src/engine.cpp:189-193). */
 YSKN_KV4_API int yskn_kv4_set_algo(int algo);
 
-/* Reads and clears the device status word of the tensor-core decode kernel on the current device (synchronises):
+/* Reads and clears the device status words of the attention kernels on the current device (synchronises):
  * 0 = ok, 1/2 = a bounded wait on the decode staging ring ran out (consumer/producer), 3 = misaligned shared memory,
  * 4/5/6 = a bounded wait ran out in the tcgen05 kernel (softmax warps / MMA issuer / producer),
- * 7 = the wait for another shard's triple ran out (yskn_kv4_merge_pushed, yskn_kv4_exchange_merge).
+ * 7 = the wait for another shard's triple ran out (yskn_kv4_merge_pushed, yskn_kv4_exchange_merge),
+ * 8/9 = a bounded wait ran out in yskn_kv4_paged_attention (rows' own part / shared part).
  * A non-zero status means the partials of that launch are invalid.  The kernels never trap; compare the reference's
  * device-side __trap() on bad input (src/kvq_gpu.cuh:91). */
 YSKN_KV4_API int yskn_kv4_device_status(int* status);
@@ -466,6 +467,7 @@ YSKN_KV4_API int yskn_kv4_paged_select(const yskn_paged_cache* c, const yskn_pag
  * sequence's tokens is never used, whatever it is.
  *   shared > 0  (a multiple of page): the first `shared` tokens lie on the same pages in the table of every row that has that many (read through the first
  *               such row's): they are read once for all rows, on the tcgen05 tensor cores, and joined with what each row has behind them.  A shorter row attends by itself.
+ *               All pages of the shared part exist (a token without one counts as a row of zeros there).
  *   ids         [rows][kvh][take], shared = 0: a row sees only the tokens of these blocks (in any order; entries outside the table, or beyond the row's last
  *               block, name none; a block named twice counts twice).
  * The sum of a row is split where the work of all rows is shared out evenly, so its last bit depends on the other rows of the call.

@@ -157,6 +157,15 @@ def test_large_scores_and_rows_of_a_wider_tensor():
         check_rows(o16, q, k, v, table, [0], [776], scale, before=before)
 
 
+@pytest.mark.parametrize("shared", [0, 160])
+def test_a_scale_of_zero_is_the_mean_of_the_values(shared):
+    k, v, table, g = make_pool([shared + 50, shared + 7], 2, 128, 32, torch.bfloat16, seed=13, garbage=True, shared=shared)
+    q = torch.randn((2, 6, 128), generator=g, device="cuda").bfloat16()
+    pos = [shared + 49, shared + 6]
+    o16, before = attend(k, v, table, ints([0, 1]), ints(pos), q, 0.0, shared=shared)
+    check_rows(o16, q, k, v, table, [0, 1], pos, 0.0, before=before)
+
+
 def test_values_that_are_not_finite_stay_in_their_channel():
     k, v, table, g = make_pool([100], 1, 128, 64, torch.float16, seed=4)
     v[int(table[0, 0]), 0, 5, 17] = float("inf")
@@ -375,6 +384,39 @@ def test_append(dt, nh, hkv, hd, page, rd, starts, rows):
             assert ((kmean[p].double() - exact).abs() <= h * exact.abs() + (1 + h) * (page * 2.0 ** -24) * k[p].double().abs().mean(1) + 2.0 ** -25).all()
             want_mean[p] = kmean[p]
     assert torch.equal(want_mean, kmean)
+
+
+def test_means_of_pages_whose_rows_come_in_any_order():
+    from yasakani_b200 import kv4, paged
+    page, dt = 32, torch.bfloat16
+    k, v, table, g = make_pool([200, 130, 64], 2, 128, page, dt, seed=21)
+    kmean = torch.full((k.shape[0], 2, 128), 5.0, dtype=dt, device="cuda")
+    rope = torch.empty((256, 64, 2), dtype=torch.float32, device="cuda")
+    kv4.launch_rope_table_g(rope, 256, 1e6, 128)
+    where = [(0, p) for p in range(37, 200)] + [(1, p) for p in range(10, 128)] + [(2, p) for p in (63, 31, 30)]     # pages that were begun before, that end inside, rows apart
+    where = [where[i] for i in torch.randperm(len(where), generator=torch.Generator().manual_seed(1)).tolist()]
+    x = torch.randn((len(where), 4, 128), generator=g, device="cuda").to(dt)
+    outs = []
+    for order in (list(range(len(where))), sorted(range(len(where)), key=lambda i: where[i])):
+        c = [t.clone() for t in (k, v, kmean)]
+        seq, pos = ints([where[i][0] for i in order]), ints([where[i][1] for i in order])
+        y = x[order].contiguous()
+        paged.launch_append(paged.PagedCache.of(*c), table, y[:, :2], y[:, 2:], seq, pos, rope, 128)
+        torch.cuda.synchronize()
+        outs.append(c)
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    full = {(s, p // page) for s, p in where if p % page == page - 1}
+    for s in range(3):
+        for b in range(table.shape[1]):
+            pg = int(table[s, b])
+            if pg < 0:
+                continue
+            if (s, b) not in full:
+                assert (outs[0][2][pg] == 5.0).all()
+                continue
+            rows = outs[0][0][pg].double()
+            h = half_step(dt)
+            assert ((outs[0][2][pg].double() - rows.mean(1)).abs() <= h * rows.mean(1).abs() + (1 + h) * page * 2.0 ** -24 * rows.abs().mean(1) + 2.0 ** -25).all(), (s, b)
 
 
 def test_append_leaves_out_rows_without_a_place():

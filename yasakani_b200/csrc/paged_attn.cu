@@ -16,9 +16,14 @@
 // each for S, share the tile's maxima and weights through shared memory (two named barriers a tile), and take HD / 4 channels each for O, so no warp holds a copy of O.
 // hd 256: one CTA an SM (192 KB in flight); hd 128: two.
 //
+// Measured (bf16, 24 / 4 heads of 256): eight rows over 2,048 .. 131,072 tokens 231 us with the merge, 6.4 TB/s of the 6.56 that a copy has; 48,000 tokens 40 us for a floor of
+// 30, in one row or in 64: 4 us from the launch to the first tile (positions, table, copy), 1 us from the last tile to the merge's start, 2 us of merge, and a
+// tail in which SMs that take in their bytes 15 % more slowly than others are left.  The tail's bytes are bound by HBM all the same: shares of the line handed out as CTAs
+// came to an end (a quarter of it, by clusterlaunchcontrol) changed 231 us to 237 and 52 to 58 (33 rows of 28 heads), for the pieces and lookups that it added.
+//
 // Tokens that a row does not see: absent blocks are read outside the tensor map (zeros); what a page holds behind the sequence's end leaves the fragments of V by a mask
 // (a weight of 0 times an infinity would be none; zeroed in shared memory it cost each row's last tile 1 us); scores are masked by selection.
-// Every wait is bounded; one that runs out sets the status word (7) and all warps walk to the end without waiting again.
+// Every wait is bounded; one that runs out sets the status word (8) and all warps walk to the end without waiting again.
 #include "paged_common.cuh"
 #include <algorithm>
 #include <cstring>
@@ -26,7 +31,7 @@
 namespace kv4 {
 namespace paged {
 
-__device__ int g_attn_status = 0;            // 0 ok; 7 = a bounded wait ran out
+__device__ int g_attn_status = 0;            // 0 ok; 8 = a bounded wait ran out
 
 namespace {
 
@@ -207,7 +212,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
       ++k;
     }
     if (!ok) {                                                         // give up; the copies under way land before the block ends
-      if (lane == 0) { atomicExch(&g_attn_status, 7); *s_abort = 1; }
+      if (lane == 0) { atomicExch(&g_attn_status, 8); *s_abort = 1; }
       for (int it = max(0, issued - NSLOT); it < issued; ++it) bar_wait(b_full + 8 * (it % NSLOT), (it / NSLOT) & 1);
       for (int it = max(0, queries - L::NQ); it < queries; ++it) bar_wait(b_qfull + 8 * (it % L::NQ), (it / L::NQ) & 1);
     }
@@ -223,9 +228,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
   constexpr int MT = HD / CW / 16;                                     // 16-channel tiles of O of this warp
   bool ok = true;
   auto wait = [&](uint32_t bar, int n) {                               // phase n of a barrier
-    if (ok && !*s_abort && bar_wait(bar, n & 1)) return;
-    if (ok) { atomicExch(&g_attn_status, 7); *s_abort = 1; }
-    ok = false;
+    if (ok && (*s_abort || !bar_wait(bar, n & 1))) { atomicExch(&g_attn_status, 8); *s_abort = 1; ok = false; }
+    __syncwarp();                                                      // each lane has polled for itself, and what follows wants the warp together
   };
   int k = 0, sg = 0, steps = first[row + 1] - first[row], head = (u0 - first[row] * kvh) / steps, at = u0 - first[row] * kvh - head * steps;
   for (int u = u0; ; ) {                                               // tiles [t0, t1) of the nt tiles of (row, kv-head)
