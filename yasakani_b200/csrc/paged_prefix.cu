@@ -150,7 +150,8 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
   cluster_sync_all();
   fence_after();
   // an allocation of all 512 columns starts at column 0: the addresses below are constants
-  if (*tmem_slot != 0 || (sb & 1023u)) { if (threadIdx.x == 0) { atomicExch(&g_prefix_status, 9); *s_abort = 1; } }
+  const bool bad = *tmem_slot != 0 || (sb & 1023u);                    // the same for the CTA; the other one's waits run out
+  if (bad && threadIdx.x == 0) { atomicExch(&g_prefix_status, 9); *s_abort = 1; }
   pdl_wait();
   pdl_launch();
 
@@ -393,10 +394,11 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
 
   if (warp < SW) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    role_softmax();
+    if (!bad) role_softmax();
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == SW) role_producer(false);
+    if (bad) {}
+    else if (warp == SW) role_producer(false);
     else if (warp == SW + 2) role_producer(true);
     else if (warp == SW + 1 && rank == 0) role_mma();
   }
