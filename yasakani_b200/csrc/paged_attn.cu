@@ -117,7 +117,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     for (int r0 = 0; r0 < P.rows; r0 += 32) {
       const int r = r0 + lane;
       int mine = 0;
-      if (r < P.rows) { const Place w = place_of(P.R, r); places[r] = w; const int nt = tiles_of(P, w); mine = nt > 0 ? nt + 1 : 0; }
+      if (r < P.rows) { const Place w = place_of<true>(P.R, r); places[r] = w; const int nt = tiles_of(P, w); mine = nt > 0 ? nt + 1 : 0; }
       int upto = mine;
       #pragma unroll
       for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, upto, d); if (lane >= d) upto += o; }
@@ -164,7 +164,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
         if (tok < w.vis) { b = (int)(tok >> P.R.lp); sub = (int)tok & (P.R.page - 1); }
       }
       if (b < 0 || b >= P.R.blocks || ((long long)b << P.R.lp) + sub >= w.vis) return x;
-      const int pg = page_of(P.R, w.seq, b);
+      const int pg = page_of<true>(P.R, w.seq, b);
       if (pg < 0) return x;
       x.at = ((pg * kvh + head) << P.R.lp) + sub;
       x.base = (b << P.R.lp) + sub;
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnP 
   if (x >= P.rows * P.nh) return;            // the same for the whole block where W is its number of warps
   const int row = x / P.nh, head = x - row * P.nh, h = head / P.g, hh = head - h * P.g, pair = row * P.R.kvh + h;
   // Ahead of the wait: the attention kernel lets this one start when all of its blocks have seen what lies in front of them finished, and writes no positions
-  const Place w = place_of(P.R, row);
+  const Place w = place_of<true>(P.R, row);
   pdl_wait();
   pdl_launch();
   if (w.seq < 0) return;

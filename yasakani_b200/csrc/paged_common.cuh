@@ -18,9 +18,11 @@ struct Rows {
 };
 
 // A row's place: sequence, and how many tokens it sees.  seq < 0: the row is padding.
+// PAST_L1: for kernels that read places and pages without a wait of their own, behind one that has waited; what an SM holds from before is then not dropped for them.
 struct Place { int seq, vis; };
-__device__ __forceinline__ Place place_of(const Rows& R, int row) {
-  const int s = R.seq[row], p = R.pos[row];
+template <bool PAST_L1 = false> __device__ __forceinline__ int read_index(const int* p) { return PAST_L1 ? __ldcg(p) : *p; }
+template <bool PAST_L1 = false> __device__ __forceinline__ Place place_of(const Rows& R, int row) {
+  const int s = read_index<PAST_L1>(R.seq + row), p = read_index<PAST_L1>(R.pos + row);
   Place w;
   w.seq = s >= 0 && s < R.seqs ? s : -1;
   const long long cap = (long long)R.blocks << R.lp;
@@ -28,8 +30,8 @@ __device__ __forceinline__ Place place_of(const Rows& R, int row) {
   return w;
 }
 // Page of block b of sequence s; -1 where the table names none.
-__device__ __forceinline__ int page_of(const Rows& R, int s, int b) {
-  const int p = R.table[(size_t)s * R.blocks + b];
+template <bool PAST_L1 = false> __device__ __forceinline__ int page_of(const Rows& R, int s, int b) {
+  const int p = read_index<PAST_L1>(R.table + (size_t)s * R.blocks + b);
   return p >= 0 && p < R.pages ? p : -1;
 }
 

@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(CT) paged_choose_kernel(const SelectP P) {
   const int row = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // Ahead of the wait, where the scores are: their kernel lets this one start when all of its blocks have seen what lies in front of them finished
   Place w{-1, 0};
-  if (P.scored) w = place_of(P.R, row);
+  if (P.scored) w = place_of<true>(P.R, row);
   pdl_wait();
   pdl_launch();
   if (!P.scored) w = place_of(P.R, row);
