@@ -536,14 +536,16 @@ int launch_paged_attention(const yskn_paged_cache& c, const yskn_paged_rows& r, 
             static_cast<uint16_t*>(a.o16) + (size_t)first * a.nh * c.hd, splits > 0 ? a.shared : 0, a.ids ? a.ids + (size_t)first * c.kvh * a.take : nullptr, a.take,
             w.span, w.ml, w.pacc, w.qml + part, w.qacc + part * c.hd, splits, splits > 0 && first == 0 ? 1 : 0};
     if (int rc = c.hd == 256 ? dispatch<256>(c, P, st) : dispatch<128>(c, P, st)) return rc;
-    // Few rows have many parts: eight warps each.  More have few: a warp, which asks for eight parts at once where there are SMs for all of them (16 rows of 28 heads over
-    // 33 blocks with their choice 33.6 us, four at once 34.7), and for four where its registers count (200 rows of 28 heads behind 5,216 tokens 62.4 us, eight 63.7)
+    // Few rows have many parts: eight warps each, a block an SM at most, since blocks of this launch lie beside the attention kernel's from early on and a second wave of them
+    // would start when all is over (five rows of 24 heads over 48 blocks with their choice 31.8 us, 240 blocks of 256 channels' halves, and 25.7 with 30).  More have few parts:
+    // a warp, which asks for eight at once where there are SMs for all of them (16 rows of 28 heads over 33 blocks 33.6 us, four at once 34.7), and for
+    // four where its registers count (200 rows of 28 heads behind 5,216 tokens 62.4 us, eight 63.7)
     const bool bf = c.dtype == YSKN_KV4_BF16;
-    const long long items = (long long)rows * a.nh;
+    const long long items = (long long)rows * a.nh * (c.hd / 128);
     const int sr = slot_rows_of(g), rc =
-        items <= 2 * SMS ? (c.hd == 256 ? launch_merge<256, 8, 8>(P, bf, sr, st) : launch_merge<128, 8, 8>(P, bf, sr, st))
-        : items * (c.hd / 128) <= 8 * SMS ? (c.hd == 256 ? launch_merge<256, 1, 8>(P, bf, sr, st) : launch_merge<128, 1, 8>(P, bf, sr, st))
-                                          : (c.hd == 256 ? launch_merge<256, 1, 4>(P, bf, sr, st) : launch_merge<128, 1, 4>(P, bf, sr, st));
+        items <= SMS ? (c.hd == 256 ? launch_merge<256, 8, 8>(P, bf, sr, st) : launch_merge<128, 8, 8>(P, bf, sr, st))
+        : items <= 8 * SMS ? (c.hd == 256 ? launch_merge<256, 1, 8>(P, bf, sr, st) : launch_merge<128, 1, 8>(P, bf, sr, st))
+                           : (c.hd == 256 ? launch_merge<256, 1, 4>(P, bf, sr, st) : launch_merge<128, 1, 4>(P, bf, sr, st));
     if (rc) return rc;
   }
   return 0;
