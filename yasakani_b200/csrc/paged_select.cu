@@ -112,7 +112,7 @@ __device__ __forceinline__ uint32_t key_of(float x) {                  // finite
 }
 __device__ __forceinline__ float float_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-constexpr int CT = 512, WARPS = CT / 32, PER = 8, BINS = 2048, LIST = 256;     // threads; blocks a thread keeps in registers
+constexpr int CT = 512, WARPS = CT / 32, BINS = 2048, LIST = 256;
 constexpr unsigned ALL = 0xffffffffu;
 struct Shared {
   uint4 range[WARPS];                        // of each warp: highest and lowest key, number of keys, largest sum of magnitudes
@@ -226,9 +226,10 @@ template <int HD, bool BF> __device__ u64 exact_key(const SelectP& P, const Plac
   return best;
 }
 
-// The choice, a block a (row, kv-head).
-template <int HD, bool BF>
-__global__ void __launch_bounds__(CT) paged_choose_kernel(const SelectP P) {
+// The choice, a thread block a (row, kv-head).  PER blocks a thread stay in registers: 8, or 32 where a table has more than 4,096 (16,383 blocks of one row read again for each walk: with
+// scores and attention 44.5 us, kept 30.5).
+template <int HD, bool BF, int PER>
+__global__ void __launch_bounds__(CT, 1) paged_choose_kernel(const SelectP P) {
   __shared__ Shared sh;
   const int row = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // Ahead of the wait, where the scores are: their kernel lets this one start when all of its blocks have seen what lies in front of them finished
@@ -241,24 +242,29 @@ __global__ void __launch_bounds__(CT) paged_choose_kernel(const SelectP P) {
   const float2* approx = P.approx + pair * P.R.blocks;
   u64* exact = P.exact + pair * P.R.blocks;
   int* ids = P.ids + pair * P.take;
-  // Block i0 + PER tid + e of the scores is x[e].  Up to PER * CT blocks are read once, beside the row's place, and stay; more are read again for each walk.
+  // A warp has 32 PER blocks in a row, x[e] of a lane is the block at 32 e + lane of them: loads of whole lines, and an order that ballots keep.  Up to PER * CT blocks are
+  // read once (few of them beside the row's place), and stay; more are read again for each walk.
   float2 x[PER];
+  const int mine0 = warp * (32 * PER) + lane;
+  const unsigned below = (1u << lane) - 1u;
   auto read = [&](int i0, int end) {
     #pragma unroll
-    for (int e = 0; e < PER; ++e) { const int i = i0 + PER * tid + e; x[e] = i < end ? approx[i] : make_float2(0.f, -1.f); }
+    for (int e = 0; e < PER; ++e) { const int i = i0 + mine0 + 32 * e; x[e] = i < end ? approx[i] : make_float2(0.f, -1.f); }
   };
-  read(0, P.R.blocks - 1);
+  if (PER == 8) read(0, P.R.blocks - 1);
   reinterpret_cast<int4*>(sh.hist)[tid] = make_int4(0, 0, 0, 0);
   if (tid == 0) sh.n = 0;
   if (w.seq < 0) return;
   const int last = w.vis > 0 ? (w.vis - 1) >> P.R.lp : -1, n = last > 0 ? last : 0;
-  #pragma unroll
-  for (int e = 0; e < PER; ++e) if (PER * tid + e >= n) x[e] = make_float2(0.f, -1.f);       // behind the candidates nothing has been written
+  if (PER == 8) {
+    #pragma unroll
+    for (int e = 0; e < PER; ++e) if (mine0 + 32 * e >= n) x[e] = make_float2(0.f, -1.f);     // behind the candidates nothing has been written
+  } else read(0, n);                                                    // a wide table may be of short rows: not ahead of the place
   auto each = [&](auto f) {
     for (int i0 = 0; i0 < n; i0 += PER * CT) {
       if (n > PER * CT) read(i0, n);
       #pragma unroll
-      for (int e = 0; e < PER; ++e) f(i0 + PER * tid + e, x[e]);
+      for (int e = 0; e < PER; ++e) f(i0 + mine0 + 32 * e, x[e]);
     }
   };
   // ---- the scores' range, the largest sum of magnitudes
@@ -299,36 +305,41 @@ __global__ void __launch_bounds__(CT) paged_choose_kernel(const SelectP P) {
   // ---- how many are chosen for sure, how many are unsure, and which those are
   int sure = 0, many = 0;
   if (!all) {
-    int mine = 0;                                                       // sure ones, and unsure ones << 16
-    each([&](int i, const float2& f) {
-      if (unsure(f)) { const int at = atomicAdd(&sh.n, 1); if (at < LIST) sh.at[at] = i; mine += 1 << 16; }
-      else if (f.y >= 0.f && f.x > hi) ++mine;
-    });
     if (n <= PER * CT) {                                                // one walk: places are known with the counts
-      const int upto = upto_lane(mine, lane);
-      if (lane == 31) sh.warps[warp] = upto;
+      int mine = 0;                                                     // sure ones, and unsure ones << 16
+      #pragma unroll
+      for (int e = 0; e < PER; ++e) if (x[e].y >= 0.f && !(x[e].x < lo)) mine += x[e].x > hi ? 1 : 1 << 16;
+      mine = __reduce_add_sync(ALL, mine);
+      if (lane == 0) sh.warps[warp] = mine;
       __syncthreads();
-      const int before = ahead_of(sh, warp, lane) + upto - mine;
-      const int total = of_all(sh, lane);
+      const int before = ahead_of(sh, warp, lane), total = of_all(sh, lane);
       sure = total & 0xffff; many = total >> 16;
       if (many <= P.take - 1 - sure) {                                  // the unsure ones are all chosen, as mostly: the border itself and nothing else
         int at = (before & 0xffff) + (before >> 16);
         #pragma unroll
-        for (int e = 0; e < PER; ++e) if (x[e].y >= 0.f && !(x[e].x < lo)) ids[at++] = PER * tid + e;
+        for (int e = 0; e < PER; ++e) {
+          const bool t = x[e].y >= 0.f && !(x[e].x < lo);
+          const unsigned b = __ballot_sync(ALL, t);
+          if (b == 0) continue;
+          if (t) ids[at + __popc(b & below)] = mine0 + 32 * e;
+          at += __popc(b);
+        }
         if (tid == 0) ids[sure + many] = last;
         for (int i = sure + many + 1 + tid; i < P.take; i += CT) ids[i] = -1;
         return;
       }
-    } else {
-      // 16 bits do not hold more: counted on their own
-      int s2 = 0;
-      each([&](int, const float2& f) { if (f.y >= 0.f && f.x > hi && !unsure(f)) ++s2; });
-      s2 = __reduce_add_sync(ALL, s2);
-      if (lane == 0) sh.warps[warp] = s2;
-      __syncthreads();
-      sure = of_all(sh, lane);
-      many = sh.n;
     }
+    int s2 = 0;                                                         // more blocks than 16 bits count, or a choice to be made among the unsure ones: which they are
+    __syncthreads();
+    each([&](int i, const float2& f) {
+      if (unsure(f)) { const int at = atomicAdd(&sh.n, 1); if (at < LIST) sh.at[at] = i; }
+      else if (f.y >= 0.f && f.x > hi) ++s2;
+    });
+    s2 = __reduce_add_sync(ALL, s2);
+    if (lane == 0) sh.warps[warp] = s2;
+    __syncthreads();
+    sure = of_all(sh, lane);
+    many = sh.n;
   }
   int left = P.take - 1 - sure;                                         // places for the unsure ones
   u64 cut = 0;                                                          // of these: above `cut`, and the first `left` equal to it
@@ -353,35 +364,40 @@ __global__ void __launch_bounds__(CT) paged_choose_kernel(const SelectP P) {
     cut = border(sh, exact, n, left);
   }
   __syncthreads();
-  // ---- one walk in rising order, PER blocks a thread
+  // ---- one walk in rising order
   int at = 0, equal = 0;                                                // taken so far; keys equal to the border so far
   for (int i0 = 0; i0 < n; i0 += PER * CT) {
     if (n > PER * CT) read(i0, n);
-    int what[PER], mine = 0;                                            // 1: taken; 1 << 16: equal to the border
+    uint32_t taken = 0, same = 0;                                       // bit e: x[e] is taken; is equal to the border
+    int mine = 0;                                                       // of the warp: taken ones, and equal ones << 16
     #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      const int i = i0 + PER * tid + e;
+      const int i = i0 + mine0 + 32 * e;
       const float2 f = x[e];
-      what[e] = 0;
+      bool t = false, q = false;
       if (f.y >= 0.f) {
-        if (all || f.x > hi) what[e] = 1;
+        if (all || f.x > hi) t = true;
         else if (unsure(f)) {
-          if (!need) what[e] = 1;
-          else if (listed) what[e] = (sh.hist[i >> 5] >> (i & 31)) & 1;
-          else { const u64 k = exact[i]; what[e] = k > cut ? 1 : k && k == cut ? 1 << 16 : 0; }
+          if (!need) t = true;
+          else if (listed) t = (sh.hist[i >> 5] >> (i & 31)) & 1;
+          else { const u64 k = exact[i]; t = k > cut; q = k && k == cut; }
         }
       }
-      mine += what[e];
+      taken |= (uint32_t)t << e; same |= (uint32_t)q << e;
+      mine += __popc(__ballot_sync(ALL, t)) + (__popc(__ballot_sync(ALL, q)) << 16);
     }
-    const int upto = upto_lane(mine, lane);
-    if (lane == 31) sh.warps[warp] = upto;
+    if (lane == 0) sh.warps[warp] = mine;
     __syncthreads();
-    const int ahead = ahead_of(sh, warp, lane) + upto - mine, total = of_all(sh, lane);
-    int a = ahead & 0xffff, e0 = equal + (ahead >> 16);
+    const int ahead = ahead_of(sh, warp, lane), total = of_all(sh, lane);
+    int e0 = equal + (ahead >> 16), place = at + (ahead & 0xffff) + min(e0, left) - min(equal, left);
     #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      if (what[e] == 1 || (what[e] > 1 && e0 < left)) ids[at + a + min(e0, left) - min(equal, left)] = i0 + PER * tid + e;
-      a += what[e] & 1; e0 += what[e] >> 16;
+      const bool q = (same >> e) & 1;
+      const unsigned bq = __ballot_sync(ALL, q);
+      const bool t = ((taken >> e) & 1) || (q && e0 + __popc(bq & below) < left);
+      const unsigned bt = __ballot_sync(ALL, t);
+      if (t) ids[place + __popc(bt & below)] = i0 + mine0 + 32 * e;
+      place += __popc(bt); e0 += __popc(bq);
     }
     at += (total & 0xffff) + min(equal + (total >> 16), left) - min(equal, left);
     equal += total >> 16;
@@ -399,7 +415,8 @@ template <int HD, bool BF> int launch(const SelectP& P, cudaStream_t st) {
     if (int rc = launch_pdl("paged_score_kernel", score, dim3((unsigned)((P.R.blocks - 1 + per - 1) / per), (unsigned)P.R.kvh, (unsigned)P.rows), SCORE_WARPS * 32, 0, st, P))
       return rc;
   }
-  return launch_pdl("paged_choose_kernel", paged_choose_kernel<HD, BF>, dim3((unsigned)P.R.kvh, (unsigned)P.rows), CT, 0, st, P);
+  auto choose = P.R.blocks <= 8 * CT ? paged_choose_kernel<HD, BF, 8> : paged_choose_kernel<HD, BF, 32>;
+  return launch_pdl("paged_choose_kernel", choose, dim3((unsigned)P.R.kvh, (unsigned)P.rows), CT, 0, st, P);
 }
 
 }  // namespace
