@@ -316,6 +316,27 @@ def test_choice_among_many_blocks(blocks, take, kind):
     assert torch.equal(ids.cpu(), choose(q, kmean, table, [0], [blocks * 16 - 1], 16, take))
 
 
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("shift", [2, 6, 10, 13])
+def test_choice_where_scores_are_differences_of_large_sums(dt, shift):
+    """Channels that cancel one another by up to 2^shift: fp32 sums are off by more than neighbours differ, and the choice is that of fp64 sums all the same."""
+    from yasakani_b200 import paged
+    hkv, nh, hd, blocks, take = 2, 6, 128, 700, 40
+    g = torch.Generator(device="cuda").manual_seed(shift)
+    km, q = torch.randn((blocks, hkv, hd), generator=g, device="cuda"), torch.randn((1, nh, hd), generator=g, device="cuda")
+    big = torch.randn((blocks, hkv, hd // 2), generator=g, device="cuda").abs() * 2.0 ** shift
+    q[..., 1::2] = q[..., ::2]
+    km[..., ::2] += big
+    km[..., 1::2] -= big
+    km, q = km.to(DT[dt]).contiguous(), q.to(DT[dt])
+    k = torch.zeros((blocks, hkv, 16, hd), dtype=DT[dt], device="cuda")
+    table = torch.randperm(blocks, generator=g, device="cuda").to(torch.int32)[None].contiguous()
+    ids = torch.empty((1, hkv, take), dtype=torch.int32, device="cuda")
+    cache = paged.PagedCache.of(k, k, km)
+    paged.launch_select(q, cache, table, ints([0]), ints([blocks * 16 - 1]), ids, paged.workspace(cache, 1, nh, blocks, select=True))
+    assert torch.equal(ids.cpu(), choose(q, km, table, [0], [blocks * 16 - 1], 16, take))
+
+
 def test_choice_among_equal_scores_takes_the_lowest_blocks():
     from yasakani_b200 import paged
     k, v, table, g = make_pool([64 * 600], 2, 128, 64, torch.float16, seed=1)
