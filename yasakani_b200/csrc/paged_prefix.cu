@@ -7,11 +7,11 @@
 //
 // A pair of CTAs (a cluster of two, cta_group::2) takes 256 (row, head) pairs of one kv-head, 128 each, and one run of the tokens in tiles of 128.  Per CTA:
 //   warps 0-7   two warpgroups that take the tiles in turn, a thread a row: scores from tensor memory, running maximum, weights back over the scores just read
-//   warps 8, 10 TMA: its half of every K tile (64 tokens), of every V tile (HD/2 channels), a box of min(page, 64) rows x 64 channels a copy, three and two stages.  A
+//   warps 8, 10 TMA: its half of every K tile (64 tokens), of every V tile (HD/2 channels), a box of min(page, 64) rows x 64 channels a copy, NK and NV stages.  A
 //               warp each, since a stage of V is free two tiles later than one of K: asked for in turn, K came a tile ahead of its use and the tensor pipe waited 780
 //               cycles a tile for it
-//   warp 9      (leader) issues S = Q K^T (M256 N128) into one of two buffers of tensor memory and O += P V (M256 N = HD, P from tensor memory)
-// Each CTA stages half a tile because an SM takes in 40 to 50 bytes a clock from L2, and a whole tile a CTA would want 64.  S of the next tile but one is issued
+//   warp 9      (leader) issues S = Q K^T (M256 N128) into one of two or three buffers of tensor memory and O += P V (M256 N = HD, P from tensor memory)
+// Each CTA stages half a tile because an SM takes in 40 to 50 bytes a clock from L2, and a whole tile a CTA would want 64.  S of a later tile is issued
 // behind P V of this one, so the tensor pipe works while the weights are computed; O is rescaled only where a maximum has grown by more than 2^8.
 //
 // Measured (bf16, 64 rows of 24 / 4 heads of 256 over 32,768 tokens, nine runs): 53 us, 51.5 GFLOP at 970 TFLOP/s; 29 tiles of 1.36 us (2,057 cycles of tensor work at 1.9 GHz
@@ -38,13 +38,15 @@ template <int HD> struct Lay {
   static constexpr int KBLK = HD / 64, VBLK = HD / 128;                // 64-channel blocks of a K half tile, of a V half tile
   static constexpr int Q_BLOCK = 128 * 128, K_BLOCK = 64 * 128, V_BLOCK = BN * 128;      // bytes: [row][128 B]
   static constexpr int K_HALF = KBLK * K_BLOCK, V_HALF = VBLK * V_BLOCK;
-  static constexpr int NK = 3, NV = 2;
+  // 128 channels: a third buffer of scores, so that S of the next tile but one does not wait for P V of this one, whose softmax takes as long as the tile's products
+  // (200 rows of 28 heads behind 5,216 tokens, with their own parts, 63.2 -> 61.9 us)
+  static constexpr int NB = HD == 128 ? 3 : 2, NK = NB + 1, NV = NB;
   static constexpr int OFF_K = KBLK * Q_BLOCK, OFF_V = OFF_K + NK * K_HALF, OFF_BAR = OFF_V + NV * V_HALF;
   static constexpr int OFF_XCH = OFF_BAR + 256;                        // float [2][128] maxima, [2][128] sums; u16 [2][128] tags
   static constexpr int TOTAL = OFF_XCH + 4 * 128 * 4 + 2 * 128 * 2;
-  static constexpr uint32_t TM_O = 2 * BN;                             // tensor memory: two score buffers of 128 columns, then O
+  static constexpr uint32_t TM_O = NB * BN;                            // tensor memory: the score buffers, 128 columns each, then O
   static constexpr int PITCH = HD * 4 + 16;                            // a row of O on its way out (eight lanes' 16 bytes on different banks)
-  static_assert(TOTAL <= 227 * 1024 && 128 * PITCH <= OFF_BAR && 2 * BN + HD <= 512, "shared memory, tensor memory");
+  static_assert(TOTAL <= 227 * 1024 && 128 * PITCH <= OFF_BAR && NB * BN + HD <= 512 && NK <= 4 && NV <= 4 && NB <= 3, "shared memory, tensor memory");
 };
 
 struct PrefixP {
@@ -123,17 +125,18 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)blockIdx.x & 1;                                // the leader (rank 0) issues the MMAs
   const int G = P.G, nquad = (P.tpc * G + 31) / 32;                    // quadrants of 32 rows that hold queries
-  // the leader's copy alone: kfull[3] vfull[2] phalf[2] pready[2] q; each CTA's: kempty[3] vempty[2] sready[2] pvdone[2]
+  // the leader's copy alone: kfull[NK] vfull[NV] phalf[NB] pready[NB] q; each CTA's: kempty[NK] vempty[NV] sready[NB] pvdone[2]
   const uint32_t b0 = sb + L::OFF_BAR;
-  const uint32_t b_kfull = b0, b_kempty = b0 + 32, b_vfull = b0 + 64, b_vempty = b0 + 80, b_sready = b0 + 96, b_pvdone = b0 + 112, b_phalf = b0 + 128,
-                 b_pready = b0 + 144, b_q = b0 + 160;
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::OFF_BAR + 168);
-  volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::OFF_BAR + 172);
+  const uint32_t b_kfull = b0, b_kempty = b0 + 32, b_vfull = b0 + 64, b_vempty = b0 + 96, b_sready = b0 + 128, b_pvdone = b0 + 152, b_phalf = b0 + 168,
+                 b_pready = b0 + 192, b_q = b0 + 216;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::OFF_BAR + 224);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::OFF_BAR + 228);
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::NK; ++i) { bar_init(b_kfull + 8 * i, 1); bar_init(b_kempty + 8 * i, 1); }
     for (int i = 0; i < L::NV; ++i) { bar_init(b_vfull + 8 * i, 1); bar_init(b_vempty + 8 * i, 1); }
-    for (int i = 0; i < 2; ++i) {
-      bar_init(b_sready + 8 * i, 1); bar_init(b_pvdone + 8 * i, 1);
+    for (int i = 0; i < 2; ++i) bar_init(b_pvdone + 8 * i, 1);
+    for (int i = 0; i < L::NB; ++i) {
+      bar_init(b_sready + 8 * i, 1);
       bar_init(b_phalf + 8 * i, 2 * nquad); bar_init(b_pready + 8 * i, 2 * nquad);          // the warps with queries of the tile's warpgroup, both CTAs
     }
     bar_init(b_q, 2 * SW);
@@ -142,7 +145,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
   }
   if (threadIdx.x < 128) reinterpret_cast<volatile uint32_t*>(smem + L::OFF_XCH + 4 * 128 * 4)[threadIdx.x] = 0;
   if (warp == SW + 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sb + L::OFF_BAR + 168), "n"(512) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sb + L::OFF_BAR + 224), "n"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   fence_before();
@@ -215,20 +218,20 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
       if (leader) {
         #pragma unroll
         for (int x = 0; x < HD / 16; ++x)
-          mma_ss((i & 1) * BN, qd + (uint64_t)(((x >> 2) * L::Q_BLOCK + (x & 3) * 32) >> 4), kd + (uint64_t)(((x >> 2) * L::K_BLOCK + (x & 3) * 32) >> 4), ID_S, x > 0);
-        commit_pair(b_sready + 8 * (i & 1));
+          mma_ss(i % L::NB * BN, qd + (uint64_t)(((x >> 2) * L::Q_BLOCK + (x & 3) * 32) >> 4), kd + (uint64_t)(((x >> 2) * L::K_BLOCK + (x & 3) * 32) >> 4), ID_S, x > 0);
+        commit_pair(b_sready + 8 * (i % L::NB));
         commit_pair(b_kempty + 8 * (i % L::NK));
       }
       __syncwarp();
     };
     auto issue_pv = [&](int i) {                                       // weights of tokens 0-63 while the others are still being computed
-      if (!wait(b_phalf + 8 * (i & 1), i >> 1) || !wait(b_vfull + 8 * (i % L::NV), i / L::NV)) return;
+      if (!wait(b_phalf + 8 * (i % L::NB), i / L::NB) || !wait(b_vfull + 8 * (i % L::NV), i / L::NV)) return;
       fence_after();
       const uint64_t vd = vd0 + (uint64_t)((i % L::NV * L::V_HALF) >> 4);
-      const uint32_t p = (i & 1) * BN;
+      const uint32_t p = i % L::NB * BN;
       #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (h == 1) { if (!wait(b_pready + 8 * (i & 1), i >> 1)) return; fence_after(); }
+        if (h == 1) { if (!wait(b_pready + 8 * (i % L::NB), i / L::NB)) return; fence_after(); }
         if (leader) {
           #pragma unroll
           for (int x = 0; x < 4; ++x) mma_ts(L::TM_O, p + 64 * h + 8 * x, vd + (uint64_t)(((4 * h + x) * 2048) >> 4), ID_PV, i > 0 || h + x > 0);
@@ -240,11 +243,10 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
     };
     wait(b_q, 0);
     fence_after();
-    if (ok) issue_s(0);
-    if (ok && n > 1) issue_s(1);
+    for (int i = 0; i < L::NB && i < n && ok; ++i) issue_s(i);
     for (int i = 0; i < n && ok; ++i) {
       issue_pv(i);
-      if (ok && i + 2 < n) issue_s(i + 2);                             // over the scores that P V of tile i has read its weights from: the pipe runs in order
+      if (ok && i + L::NB < n) issue_s(i + L::NB);                     // over the scores that P V of tile i has read its weights from: the pipe runs in order
     }
   };
 
@@ -286,8 +288,9 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
     bool ok = true;
     #pragma unroll 1
     for (int i = hf; i < n; i += 2) {
-      const uint32_t sc = trow + hf * BN;
-      if (!bar_wait(b_sready + 8 * hf, (i >> 1) & 1)) { fail(); ok = false; }
+      const int sbuf = i % L::NB;            // of three buffers a warpgroup sees every other phase; the one between is over, since S of this warpgroup's tile before came behind it
+      const uint32_t sc = trow + sbuf * BN;
+      if (!bar_wait(b_sready + 8 * sbuf, (i / L::NB) & 1)) { fail(); ok = false; }
       if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
       fence_after();
       uint32_t xr[128];
@@ -351,7 +354,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
           tm_wait_st();
           fence_before();
           __syncwarp();
-          if (lane == 0) arrive_cluster((c == 1 ? lead_half : lead_ready) + 8 * (i & 1));
+          if (lane == 0) arrive_cluster((c == 1 ? lead_half : lead_ready) + 8 * sbuf);
         }
       }
       l += (s0.x + s0.y) + (s1.x + s1.y);
