@@ -169,3 +169,27 @@ def test_a_cache_on_another_device_than_the_current_one():
     torch.cuda.synchronize(1)
     assert torch.cuda.current_device() == 0
     check_rows(*(t.to("cuda:0") for t in (o, q, k, v, table)), seq.tolist(), pos.tolist(), 0.09)
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("tiles", range(1, 10))
+def test_prefix_runs_of_few_tiles_from_cold_caches(hd, tiles):
+    """Each number of 128-token tiles in a run meets another phase of the prefix kernel's buffers at its end.  160 rows of 8 heads over 8 shared heads are 40
+    pairs of blocks, more than half of those that fit, so a run has all the tiles; keys and values come from memory, late, and each launch has the same bits."""
+    from yasakani_b200 import kv4, paged
+    rows, nh, hkv, page, shared = 160, 64, 8, 32, 128 * tiles - 32 * (tiles % 2)
+    k, v, _, table, seq, pos, q = case(lengths=[shared + 1 + i % 3 for i in range(rows)], nh=nh, hkv=hkv, hd=hd, page=page, shared=shared, seed=tiles)
+    cache, ws = paged.PagedCache.of(k, v), paged.workspace(paged.PagedCache.of(k, v), rows, nh, table.shape[1], shared=shared)
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    outs = []
+    for i in range(12):
+        o = torch.full_like(q, 7.0)
+        ws.fill_(0xFF)                                           # NaN wherever nothing is written
+        flush.fill_(i)
+        paged.launch_attention(q, cache, table, seq, pos, 0.09, o, ws, shared=shared)
+        outs.append(o)
+    torch.cuda.synchronize()
+    assert kv4.device_status() == 0
+    assert all(torch.equal(o.view(torch.int16), outs[0].view(torch.int16)) for o in outs)
+    some = torch.tensor([0, 1, 15, 16, 31, 32, 80, 127, 159], device="cuda")
+    check_rows(outs[0][some], q[some], k, v, table, seq[some], pos[some], 0.09)

@@ -126,18 +126,17 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)blockIdx.x & 1;                                // the leader (rank 0) issues the MMAs
   const int G = P.G, nquad = (P.tpc * G + 31) / 32;                    // quadrants of 32 rows that hold queries
-  // the leader's copy alone: kfull[NK] vfull[NV] phalf[NB] pready[NB] q; each CTA's: kempty[NK] vempty[NV] sready[NB] pvdone[2]
+  // the leader's copy alone: kfull[NK] vfull[NV] phalf[NB] pready[NB] q; each CTA's: kempty[NK] vempty[NV] sready[NB] pvdone[NB]
   const uint32_t b0 = sb + L::OFF_BAR;
-  const uint32_t b_kfull = b0, b_kempty = b0 + 32, b_vfull = b0 + 64, b_vempty = b0 + 96, b_sready = b0 + 128, b_pvdone = b0 + 152, b_phalf = b0 + 168,
-                 b_pready = b0 + 192, b_q = b0 + 216;
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::OFF_BAR + 224);
-  volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::OFF_BAR + 228);
+  const uint32_t b_kfull = b0, b_kempty = b0 + 32, b_vfull = b0 + 64, b_vempty = b0 + 96, b_sready = b0 + 128, b_pvdone = b0 + 152, b_phalf = b0 + 176,
+                 b_pready = b0 + 200, b_q = b0 + 224;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::OFF_BAR + 232);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(smem + L::OFF_BAR + 236);
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::NK; ++i) { bar_init(b_kfull + 8 * i, 1); bar_init(b_kempty + 8 * i, 1); }
     for (int i = 0; i < L::NV; ++i) { bar_init(b_vfull + 8 * i, 1); bar_init(b_vempty + 8 * i, 1); }
-    for (int i = 0; i < 2; ++i) bar_init(b_pvdone + 8 * i, 1);
     for (int i = 0; i < L::NB; ++i) {
-      bar_init(b_sready + 8 * i, 1);
+      bar_init(b_sready + 8 * i, 1); bar_init(b_pvdone + 8 * i, 1);
       bar_init(b_phalf + 8 * i, 2 * nquad); bar_init(b_pready + 8 * i, 2 * nquad);          // the warps with queries of the tile's warpgroup, both CTAs
     }
     bar_init(b_q, 2 * SW);
@@ -146,7 +145,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
   }
   if (threadIdx.x < 128) reinterpret_cast<volatile uint32_t*>(smem + L::OFF_XCH + 4 * 128 * 4)[threadIdx.x] = 0;
   if (warp == SW + 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sb + L::OFF_BAR + 224), "n"(512) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sb + L::OFF_BAR + 232), "n"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   fence_before();
@@ -239,7 +238,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
         }
         __syncwarp();
       }
-      if (leader) { commit_pair(b_pvdone + 8 * (i & 1)); commit_pair(b_vempty + 8 * (i % L::NV)); }
+      if (leader) { commit_pair(b_pvdone + 8 * (i % L::NB)); commit_pair(b_vempty + 8 * (i % L::NV)); }
       __syncwarp();
     };
     wait(b_q, 0);
@@ -325,7 +324,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
       xtag[hf * 128 + rho] = (uint16_t)(i + 1);
       if (mown != m) { l *= ex2(mown - m); mown = m; }
       if (__any_sync(0xffffffffu, bump && i > 0)) {                    // rows whose maximum stays multiply by exactly 1
-        if (!bar_wait(b_pvdone + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1)) { fail(); ok = false; }
+        if (!bar_wait(b_pvdone + 8 * ((i - 1) % L::NB), ((i - 1) / L::NB) & 1)) { fail(); ok = false; }
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         fence_after();
         #pragma unroll 1
@@ -370,7 +369,8 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_const
       if (ok) ok = tag_wait(hf ^ 1, n + 1);
       l = xval[256 + rho] + xval[256 + 128 + rho];
     }
-    if (ok && !bar_wait(b_pvdone + 8 * ((n - 1) & 1), ((n - 1) >> 1) & 1)) ok = false;
+    // one barrier a score buffer: its phase before this is tile n - 1 - NB's, over since S of tile n - 1 came behind that P V and a tag of that S was seen
+    if (ok && !bar_wait(b_pvdone + 8 * ((n - 1) % L::NB), ((n - 1) / L::NB) & 1)) ok = false;
     if (!ok) fail();
     if (!__all_sync(0xffffffffu, ok && !*s_abort)) return;
     fence_after();
