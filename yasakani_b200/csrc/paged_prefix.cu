@@ -39,8 +39,7 @@ template <int HD> struct Lay {
   static constexpr int Q_BLOCK = 128 * 128, K_BLOCK = 64 * 128, V_BLOCK = BN * 128;      // bytes: [row][128 B]
   static constexpr int K_HALF = KBLK * K_BLOCK, V_HALF = VBLK * V_BLOCK;
   // 128 channels: a third buffer of scores, so that S of the next tile but one does not wait for P V of this one, whose softmax takes as long as the tile's products
-  // (200 rows of 28 heads behind 5,216 tokens, with their own parts, 62.7 -> 61.1 us;
-  // this kernel alone 24.4 -> 23.1)
+  // (200 rows of 28 heads behind 5,216 tokens, with their own parts, 63.3 -> 62.1 us)
   static constexpr int NB = HD == 128 ? 3 : 2, NK = NB + 1, NV = NB;
   static constexpr int OFF_K = KBLK * Q_BLOCK, OFF_V = OFF_K + NK * K_HALF, OFF_BAR = OFF_V + NV * V_HALF;
   static constexpr int OFF_XCH = OFF_BAR + 256;                        // float [2][128] maxima, [2][128] sums; u16 [2][128] tags
