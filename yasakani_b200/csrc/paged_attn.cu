@@ -1,6 +1,9 @@
 // Attention of single rows over a paged 16-bit cache (sm_100a): batched decode, attention over chosen blocks, the rows' own part behind a shared prefix.
 //
 // Mathematics: o = sum_j p_j v_j / sum_j p_j, p_j = 2^(s q.k_j log2 e - m), m the running maximum; a tile of 64 tokens at a time, one pass over K and V.
+// p is rounded to the cache's type for the product with V, its sum stays fp32.  fp16 has no numbers between 0 and 2^-24 and less than 11 bits below 2^-14, and a long tail of
+// such weights may carry a channel in which the largest weight's value is zero: there m is the maximum less 15, so that p lies in (0, 2^15] and is rounded by half a step of its own down to 2^-29 of
+// the largest, by 2^-40 of that below.  It cancels in the quotient, and the merge takes (m, l, O) as it takes others.
 //
 // Bound: HBM.  A token of a kv-head costs 4 HD bytes and 2 G HD multiply-adds for the G <= 16 heads that share it, which is what warp-level tensor-core
 // tiles are for: S^T[16 tokens x 8 heads] = K Q^T, O^T[16 channels x 8 heads] += V^T P^T, keys and values straight from the swizzled tiles (ldmatrix).
@@ -38,6 +41,7 @@ namespace {
 constexpr int ROWS = 224;                    // rows of one launch (a multiple of 32; what shared memory leaves beside the ring)
 constexpr int NSLOT = 6;                     // half stages of the ring: K, V, K, V, K, V
 constexpr int CW = 4, NT_ = (CW + 1) * 32;   // compute warps; threads
+template <bool BF> constexpr float ABOVE = BF ? 0.f : 15.f;            // log2 of the largest weight
 
 struct AttnP {
   Rows R; int rows, g, nh;
@@ -295,7 +299,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
           float v = fmaxf(x[n][e], x[n][e + 2]);
           #pragma unroll
           for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-          if (lane < 4) smax[(buf * CW + warp) * (NT * 8) + n * 8 + 2 * j + e] = v;
+          if (lane < 4) smax[(buf * CW + warp) * (NT * 8) + n * 8 + 2 * j + e] = v - ABOVE<BF>;
         }
       }
       __syncwarp();
@@ -315,7 +319,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
         m[n][0] = top.x; m[n][1] = top.y;
         const float p0 = ex2(x[n][0] - r0), p1 = ex2(x[n][1] - r1), p2 = ex2(x[n][2] - r0), p3 = ex2(x[n][3] - r1);
         l[n][0] = l[n][0] * alpha[n][0] + (p0 + p2); l[n][1] = l[n][1] * alpha[n][1] + (p1 + p3);
-        stm2t(sb + L::OFF_P + (buf * NT * 8 + n * 8 + (lane & 7)) * L::PP + (tok + 8 * ((lane >> 3) & 1)) * 2, pack16<BF>(p0, p1), pack16<BF>(p2, p3));
+        stm2t(sb + L::OFF_P + (buf * NT * 8 + n * 8 + (lane & 7)) * L::PP + (tok + 8 * ((lane >> 3) & 1)) * 2, pack_weights<BF>(p0, p1), pack_weights<BF>(p2, p3));
       }
       // ---- O^T of this warp's channels
       wait(b_full + 8 * vslot, iv / NSLOT);

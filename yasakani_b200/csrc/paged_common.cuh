@@ -70,6 +70,13 @@ template <bool BF> __device__ __forceinline__ uint32_t pack16(float lo, float hi
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
+// Two weights of a softmax rounded to the 16-bit type.  fp16's largest number stands for what is beyond it, as only scores have whose own steps are of that size.
+template <bool BF> __device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
+  if (BF) return pack16<true>(lo, hi);
+  uint32_t d;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
 template <bool BF> __device__ __forceinline__ float2 unpack16(uint32_t w) {
   if (BF) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   const __half2 h = *reinterpret_cast<const __half2*>(&w);
