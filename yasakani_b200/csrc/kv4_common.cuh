@@ -41,14 +41,23 @@ inline int launch_pdl(const char* who, K kern, dim3 grid, int threads, size_t sm
   return launch_status(who);
 }
 
-// Function attributes are per device: true the first time a launcher runs on the current device (flags = one word per
+// Function attributes are per device: `set` (0 = done) runs the first time a launcher is used on the current device (flags = one word per
 // launcher, bit d = done on device d).  The reference sets them once per process (src/q35_fa.cu:305-307) because an engine
-// owns one GPU; a process that drives several GPUs through this library gets them on each.
-inline bool first_use_on_device(std::atomic<unsigned long long>& flags) {
+// owns one GPU; a process that drives several GPUs through this library gets them on each.  The bit appears when `set` has done its work:
+// threads that come at the same time set the attributes twice, which changes nothing, none launches without them, and one that failed is tried again.
+template <class F> inline int once_for_bit(std::atomic<unsigned long long>& flags, unsigned long long bit, F set) {
+  if (flags.load(std::memory_order_acquire) & bit) return 0;
+  if (int rc = set()) return rc;
+  flags.fetch_or(bit, std::memory_order_release);
+  return 0;
+}
+template <class F> inline int once_per_device(std::atomic<unsigned long long>& flags, F set) {
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return true;
-  const unsigned long long bit = 1ull << dev;
-  return (flags.fetch_or(bit) & bit) == 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return set();
+  return once_for_bit(flags, 1ull << dev, set);
+}
+template <class K> inline int allow_smem(std::atomic<unsigned long long>& flags, K kern, size_t bytes) {       // dynamic shared memory beyond 48 KB
+  return once_per_device(flags, [&] { KV4_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes)); return 0; });
 }
 
 // ---- device scalar helpers ----

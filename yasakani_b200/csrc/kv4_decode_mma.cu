@@ -801,10 +801,12 @@ int launch_m(const yskn_attn_g_args& a, int g, Shard sh, int early, const yskn_k
   using L = Lay<HD, RD, Q>;
   auto kern = kv4_decode_mma_kernel<HD, RD, DT, Q, multi>;
   static std::atomic<unsigned long long> attr{0};               // once per device, like the reference's launchers once per process
-  if (first_use_on_device(attr)) {
+  const int rc = once_per_device(attr, [&] {
     KV4_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
     KV4_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-  }
+    return 0;
+  });
+  if (rc) return rc;
   DecodeP P{a, sh, g, early, ms};
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.splits, a.kvh, a.M); cfg.blockDim = dim3(NTHREADS); cfg.dynamicSmemBytes = L::TOTAL; cfg.stream = st;

@@ -1565,7 +1565,7 @@ int launch_tc_hd(const yskn_attn_g_args& a, int g, int rd, int bf16, const TcWs&
     KV4_REJECT("yskn_kv4_attention_tc: cuTensorMapEncodeTiled failed or is unavailable");
   auto kern = bf16 ? kv4_tc_attn_kernel<HD, 3> : kv4_tc_attn_kernel<HD, 0>;
   static std::atomic<unsigned long long> attr[2] = {{0}, {0}};
-  if (first_use_on_device(attr[bf16 != 0])) KV4_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+  if (int rc = allow_smem(attr[bf16 != 0], kern, L::TOTAL)) return rc;
   int tpc; const int qtiles = tc_tiles(a.M, g, false, &tpc);
   TcP P{a.d_pos, a.M, a.splits, g, tpc, a.nh, a.max_ctx, w.ks_rows, a.qscale, a.pm, a.pl, a.pacc, o16, bv, a.kv, a.rope, rd,
         static_cast<const uint16_t*>(a.q16), bf16, nullptr, nullptr, nullptr, nullptr};
@@ -1581,7 +1581,7 @@ int launch_tc_fused_hd(const yskn_attn_g_args& a, int g, int rd, int bf16, uint1
   memset(&mq, 0, sizeof(mq));
   auto kern = kv4_tc_attn_kernel<HD, 1>;
   static std::atomic<unsigned long long> attr{0};
-  if (first_use_on_device(attr)) KV4_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+  if (int rc = allow_smem(attr, kern, L::TOTAL)) return rc;
   // The tiles that a pair's own tokens lie in are converted twice.  Where the tokens of a pair are a whole part of a key tile (2, 4 or 8 heads a kv-head), even shares of
   // more than a tile of tokens lie across one tile more.  Rows of eight heads of 128 channels, one split, us from position 0 and behind 2,500 tokens: 150 rows 20.6 and
   // 61.2 with whole shares before the requests a tile ahead, 21.6 and 59.1 with them and even shares, 19.3 and 60.7 with whole ones; 300 rows 23.1 and 63.9, 23.9 and
@@ -1653,7 +1653,7 @@ int launch_kv8_attention_tc(const yskn_kv8_attn_args& a, int act_dtype, cudaStre
   memset(&mq, 0, sizeof(mq));
   auto kern = kv4_tc_attn_kernel<256, 2>;
   static std::atomic<unsigned long long> attr{0};
-  if (first_use_on_device(attr)) KV4_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+  if (int rc = allow_smem(attr, kern, L::TOTAL)) return rc;
   int tpc; const int qtiles = tc_tiles(a.M, g, true, &tpc);
   TcP P{a.d_pos, a.M, a.splits, g, tpc, a.nh, a.max_ctx, 0, a.qscale, a.pm, a.pl, a.pacc, nullptr, nullptr, yskn_kv_layer{}, nullptr, 0,
         a.q16, bf16, a.k8, a.v8, a.ks, a.vs};
@@ -1681,7 +1681,7 @@ int launch_kv8_attention_tc_ws(const yskn_kv8_attn_args& a, int act_dtype, void*
     KV4_REJECT("yskn_kv8_attention_ws: cuTensorMapEncodeTiled failed or is unavailable");
   auto kern = kv4_tc_attn_kernel<256, 4>;
   static std::atomic<unsigned long long> attr{0};
-  if (first_use_on_device(attr)) KV4_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+  if (int rc = allow_smem(attr, kern, L::TOTAL)) return rc;
   int tpc; const int qtiles = tc_tiles(a.M, g, true, &tpc);
   TcP P{a.d_pos, a.M, a.splits, g, tpc, a.nh, a.max_ctx, 0, a.qscale, a.pm, a.pl, a.pacc, nullptr, nullptr, yskn_kv_layer{}, nullptr, 0,
         a.q16, act_dtype == YSKN_KV4_BF16, nullptr, nullptr, nullptr, nullptr};

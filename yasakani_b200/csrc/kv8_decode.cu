@@ -441,12 +441,12 @@ int launch_kv8_attention(const yskn_kv8_attn_args& a, int act_dtype, cudaStream_
   const dim3 grid(a.splits, a.kvh, a.M);
   if (act_dtype == YSKN_KV4_BF16) {
     static std::atomic<unsigned long long> attr{0};
-    if (first_use_on_device(attr)) KV4_CUDA(cudaFuncSetAttribute(kv8_decode_kernel<YSKN_KV4_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (int rc = allow_smem(attr, kv8_decode_kernel<YSKN_KV4_BF16>, smem)) return rc;
     return launch_pdl("kv8_decode_kernel", kv8_decode_kernel<YSKN_KV4_BF16>, grid, KV8_WARPS * 32, smem, st, P);
   }
   if (act_dtype == YSKN_KV4_F16) {
     static std::atomic<unsigned long long> attr{0};
-    if (first_use_on_device(attr)) KV4_CUDA(cudaFuncSetAttribute(kv8_decode_kernel<YSKN_KV4_F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (int rc = allow_smem(attr, kv8_decode_kernel<YSKN_KV4_F16>, smem)) return rc;
     return launch_pdl("kv8_decode_kernel", kv8_decode_kernel<YSKN_KV4_F16>, grid, KV8_WARPS * 32, smem, st, P);
   }
   KV4_REJECT("yskn_kv8_attention: q16 is bf16 or fp16 (act_dtype %d)", act_dtype);

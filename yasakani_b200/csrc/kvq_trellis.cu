@@ -944,11 +944,13 @@ int launch_tb_encode(const uint8_t* blob, int nm, const float* x, const int* grp
   if (rows <= 0 || nm < 1 || nm > TB_NM) KV4_REJECT("yskn_tb_encode: bad shape (rows %d, multipliers %d)", rows, nm);
   if (pay && (pay_stride < 160 || pay_stride % 4 || ((uintptr_t)pay & 3))) KV4_REJECT("yskn_tb_encode: payload rows need a stride of at least 160 bytes, a multiple of 4");
   static std::atomic<unsigned long long> attr{0};
-  if (first_use_on_device(attr)) {
+  const int rc = once_per_device(attr, [] {
     KV4_CUDA(cudaFuncSetAttribute(tb_encode_kernel<TB_WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TbRowSmem::bytes(TB_NM, TB_WIDE)));
     KV4_CUDA(cudaFuncSetAttribute(tb_encode_kernel<TB_NARROW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TbRowSmem::bytes(TB_NM, TB_NARROW)));
     KV4_CUDA(cudaFuncSetAttribute(tb_encode_kernel<TB_ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TbRowSmem::bytes(1, TB_ONE)));
-  }
+    return 0;
+  });
+  if (rc) return rc;
   const TbP P{blob, nm, x, grp, pos, rows, y, pay, pay_stride, side, whole};
   const int most = nm == 1 ? TB_ONE : rows <= TB_WIDE_ROWS ? TB_WIDE : TB_NARROW;
   auto kern = most == TB_ONE ? tb_encode_kernel<TB_ONE> : most == TB_WIDE ? tb_encode_kernel<TB_WIDE> : tb_encode_kernel<TB_NARROW>;
@@ -967,12 +969,12 @@ int launch_tb_attention(const yskn_tb_attn_args& a, int act_dtype, cudaStream_t 
   const dim3 grid(a.splits, a.kvh, a.M);
   if (act_dtype == YSKN_KV4_BF16) {
     static std::atomic<unsigned long long> attr{0};
-    if (first_use_on_device(attr)) KV4_CUDA(cudaFuncSetAttribute(tb_attn_kernel<YSKN_KV4_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (int rc = allow_smem(attr, tb_attn_kernel<YSKN_KV4_BF16>, smem)) return rc;
     return launch_pdl("tb_attn_kernel", tb_attn_kernel<YSKN_KV4_BF16>, grid, TBA_WARPS * 32, smem, st, P);
   }
   if (act_dtype == YSKN_KV4_F16) {
     static std::atomic<unsigned long long> attr{0};
-    if (first_use_on_device(attr)) KV4_CUDA(cudaFuncSetAttribute(tb_attn_kernel<YSKN_KV4_F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (int rc = allow_smem(attr, tb_attn_kernel<YSKN_KV4_F16>, smem)) return rc;
     return launch_pdl("tb_attn_kernel", tb_attn_kernel<YSKN_KV4_F16>, grid, TBA_WARPS * 32, smem, st, P);
   }
   KV4_REJECT("yskn_tb_attention: q16 is bf16 or fp16 (act_dtype %d)", act_dtype);

@@ -500,7 +500,7 @@ int launch(const yskn_paged_cache& c, const AttnP& P, cudaStream_t st) {
   using L = Lay<HD, NT>;
   auto kern = paged_attn_kernel<HD, NT, BF>;
   static std::atomic<unsigned long long> attr{0};
-  if (first_use_on_device(attr)) KV4_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+  if (int rc = allow_smem(attr, kern, L::TOTAL)) return rc;
   CUtensorMap mk, mv;
   memcpy(&mk, c.maps[0], sizeof(mk)); memcpy(&mv, c.maps[1], sizeof(mv));
   return launch_pdl("paged_attn_kernel", kern, dim3((unsigned)ctas_of(HD)), NT_, L::TOTAL, st, mk, mv, P);

@@ -432,7 +432,7 @@ int launch(const yskn_paged_cache& c, const PrefixP& P, int pairs, cudaStream_t 
   using L = Lay<HD>;
   auto kern = paged_prefix_kernel<HD, BF>;
   static std::atomic<unsigned long long> attr{0};
-  if (first_use_on_device(attr)) KV4_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
+  if (int rc = allow_smem(attr, kern, L::TOTAL)) return rc;
   CUtensorMap mk, mv;
   memcpy(&mk, c.maps[2], sizeof(mk)); memcpy(&mv, c.maps[3], sizeof(mv));
   return launch_pdl("paged_prefix_kernel", kern, dim3(2u * pairs, (unsigned)P.splits, (unsigned)c.kvh), THREADS, L::TOTAL, st, mk, mv, P);
