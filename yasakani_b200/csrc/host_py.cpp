@@ -360,8 +360,10 @@ FN(paged_append) {                                       // cache, keys, table, 
     if (v[7] != Py_None) {
       const at::Tensor& rope = paged_tensor(P, v[7], at::kFloat, "rope");
       check_dev(rope, "rope");
-      if (a.rd > 0) {                                    // [positions][rd / 2][2], or flat
-        if (rope.numel() % a.rd || rope.numel() / a.rd > INT_MAX) fail(PyExc_ValueError, "rope: fp32 [positions][rd / 2][2]");
+      if (a.rd > 0) {                                    // [positions][rd / 2][2], [positions][rd] or flat: a table of another width would be read as one of more positions
+        const int64_t d = rope.dim();
+        const bool fits = d == 3 ? rope.size(1) == a.rd / 2 && rope.size(2) == 2 : d == 2 ? rope.size(1) == a.rd : d == 1 && rope.numel() % a.rd == 0;
+        if (!fits || rope.numel() / a.rd > INT_MAX) fail(PyExc_ValueError, "rope: fp32 [positions][rd / 2][2]");
         a.rope = (const float*)rope.data_ptr(); a.rope_rows = (int)(rope.numel() / a.rd);
       }
     }

@@ -67,7 +67,8 @@ def workspace(cache: PagedCache, rows: int, nh: int, blocks: int, shared: int = 
 def launch_append(cache: PagedCache, table, k, v, seq, pos, rope=None, rd: int = 0, q=None, q_out=None, stream=None) -> None:
     """Rotates keys (and queries, into q_out) at each row's position and writes keys and values into their pages, mean keys of pages that
     are full with these rows too (yskn_kv4_paged_append).  k, v [rows][hkv][hd], q [rows][nh][hd] in the cache's type; rows may be slices of a wider
-    tensor (their heads are contiguous).  rope: fp32 [positions][rd / 2][2] as kv4.launch_rope_table_g writes it."""
+    tensor (their heads are contiguous).  rope: fp32 [positions][rd / 2][2] as kv4.launch_rope_table_g writes it,
+    or the same numbers as [positions][rd] or flat; a table of another rotary width is refused."""
     host.paged_append(cache.c, cache.k, table, k, v, seq, pos, rope, rd, q, q_out, stream)
 
 
