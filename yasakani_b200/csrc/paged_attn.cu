@@ -144,11 +144,11 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
     // =========================================================================================== producer
     const int none = (P.R.pages * kvh) << P.R.lp;                      // a row outside the arrays: zeros
     // Boxes come 32 at a time, one a lane, looked up a batch ahead and across the borders of pairs: the lookups' latency (place, chosen block, table) is never
-    // waited for.  A box: its row in the arrays, the position of its first token (no token: INT_MAX), its pair.
+    // waited for.  A box: its row in the arrays, the position of its first token, its pair.
     struct Box { int at, base, pair; };
     int base_row = row;                                                // of the steps that are looked up: they lie a few rows on at most
     auto box_of = [&](int u, int j) {                                  // box j of step u; of a step without a tile: pair -1
-      Box x{none, 0x7fffffff, -1};
+      Box x{none, NO_TOKEN, -1};
       if (u >= u1) return x;
       int row = base_row;
       #pragma unroll 1
@@ -268,7 +268,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
       wait(b_full + 8 * kslot, ik / NSLOT);
       const int tok = 16 * warp, cb = tok >> lc, rr = tok & (chunk - 1);                    // its chunk, first row there
       const int4 b4 = *reinterpret_cast<const int4*>(smem + L::OFF_BASE + (k % 3) * 16);    // read before the half stage is handed back: the next tile's come then
-      auto base_of = [&](int i) { return i == 0 ? b4.x : i == 1 ? b4.y : i == 2 ? b4.z : b4.w; };
+      auto base_of = [&](int i) { return box_base(i == 0 ? b4.x : i == 1 ? b4.y : i == 2 ? b4.z : b4.w, w.vis); };
       const int base = base_of(cb);
       float c[NT][2][4];                                                                    // two sums, so that products do not wait for one another
       #pragma unroll
@@ -288,7 +288,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
         }
       }
       // tokens of the tile that the row sees: lane row g8 and g8 + 8 of this warp's
-      const bool see0 = base != 0x7fffffff && base + rr + g8 < w.vis, see1 = base != 0x7fffffff && base + rr + g8 + 8 < w.vis;
+      const bool see0 = base + rr + g8 < w.vis, see1 = base + rr + g8 + 8 < w.vis;
       float x[NT][4];
       #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -339,7 +339,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
           const int t16 = 32 * h + 16 * ks, ch = t16 >> lc, r16 = t16 & (chunk - 1), r = r16 + (lane & 7) + ((lane >> 4) & 1) * 8;
           // of these 16 tokens the row sees the first n16 (no block: none, and what was read is zero); a lane's registers hold tokens 2j, 2j + 1 and the eight behind them
           const int n16 = w.vis - base_of(ch) - r16 - 2 * j;
-          const uint32_t keep0 = (n16 > 0 ? 0xffffu : 0u) | (n16 > 1 ? 0xffff0000u : 0u), keep1 = (n16 > 8 ? 0xffffu : 0u) | (n16 > 9 ? 0xffff0000u : 0u);
+          const uint32_t keep0 = keep_pair(n16), keep1 = keep_pair(n16 - 8);
           #pragma unroll
           for (int y = 0; y < MT; ++y) {
             const int cc = warp * (2 * MT) + 2 * y + ((lane >> 3) & 1);

@@ -35,6 +35,12 @@ template <bool PAST_L1 = false> __device__ __forceinline__ int page_of(const Row
   return p >= 0 && p < R.pages ? p : -1;
 }
 
+// A box's first token for a row that sees `vis` tokens.  One without a token of the row's (NO_TOKEN among them) stands at `vis`, so that offsets into it can be added.
+constexpr int NO_TOKEN = 0x7fffffff;
+__host__ __device__ __forceinline__ int box_base(int base, int vis) { return base < vis ? base : vis; }
+// Of two 16-bit values in a register, tokens 0 and 1 of the n that the row still sees from there: those that it sees.
+__host__ __device__ __forceinline__ uint32_t keep_pair(int n) { return (n > 0 ? 0xffffu : 0u) | (n > 1 ? 0xffff0000u : 0u); }
+
 // ---------------------------------------------------------------------------------------------------------------- PTX
 constexpr uint32_t WAIT_LIMIT = 1u << 22;    // polls before a wait gives up
 __device__ __forceinline__ uint32_t s_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
