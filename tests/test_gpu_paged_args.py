@@ -42,3 +42,16 @@ def test_angles_in_any_of_their_shapes():
         paged.launch_append(**dict(a, rope=a["rope"].view(shape)))
         outs.append((k, v, q_out))
     assert all(torch.equal(x, y) for o in outs for x, y in zip(o, outs[0])) and not (outs[0][2] == 7.0).any()
+
+
+def test_an_output_without_its_queries_is_refused():
+    from yasakani_b200 import paged
+    a, k, v, q_out = append_case(64)
+    old = k.clone()
+    with pytest.raises(ValueError, match="q_out"):
+        paged.launch_append(**dict(a, q=None))
+    torch.cuda.synchronize()
+    assert torch.equal(k, old) and (q_out == 7.0).all()
+    paged.launch_append(**dict(a, q=None, q_out=None))
+    torch.cuda.synchronize()
+    assert not torch.equal(k, old)

@@ -371,7 +371,7 @@ FN(paged_append) {                                       // cache, keys, table, 
       const HeadRows q = head_rows(P, v[9], -1, "q"), out = head_rows(P, v[10], q.heads, "q_out");
       check_dev(tensor(v[10], "q_out"), "q_out");
       a.q_in = q.p; a.q_out = out.p; a.q_stride = q.stride; a.nh = q.heads;
-    }
+    } else if (v[10] != Py_None) fail(PyExc_ValueError, "q_out without q: nothing would be written to it");
     return paged_call(P, v[11], "yskn_kv4_paged_append", [&](cudaStream_t st) { return yskn_kv4_paged_append(&P.c, &P.r, &a, st); });
   });
 }
