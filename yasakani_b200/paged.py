@@ -25,7 +25,12 @@ from .kv4 import _dtype_code
 
 
 class PagedCache:
-    """One layer's pages: k, v [pages][hkv][page][hd], and with `means` kmean [pages][hkv][hd], the mean key of every page that has been filled."""
+    """One layer's pages: k, v [pages][hkv][page][hd], and with `means` kmean [pages][hkv][hd], the mean key of every page that has been filled.
+    What the tensors hold may be written by anyone; the tensors themselves stay those of the start, whose addresses the tensor maps hold (`of` makes a cache over others)."""
+
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    kmean = property(lambda self: self._kmean)
 
     def __init__(self, pages: int, hkv: int, hd: int, page: int = 64, dtype=torch.bfloat16, means: bool = False, device="cuda"):
         z = lambda *shape: torch.zeros(shape, dtype=dtype, device=device)
@@ -45,7 +50,7 @@ class PagedCache:
             raise TypeError("k, v and kmean are all fp16 or all bf16, on one device")
         if not all(t.is_cuda and t.is_contiguous() for t in (k, v, kmean) if t is not None):
             raise AssertionError("device buffers must be contiguous CUDA tensors")
-        self.k, self.v, self.kmean = k, v, kmean
+        self._k, self._v, self._kmean = k, v, kmean
         self.pages, self.hkv, self.page, self.hd = k.shape
         self.dtype, self.device = k.dtype, k.device
         self.c = PagedCacheC(k.data_ptr(), v.data_ptr(), kmean.data_ptr() if kmean is not None else None, self.pages, self.hkv, self.page, self.hd, _dtype_code(k))
