@@ -64,7 +64,7 @@ __device__ void page_means(const AppendP& P, int r0, int h) {
   __shared__ int from[128];                                            // the row of this call that holds a token of the page; -1: the cache does
   const int tid = threadIdx.x, lane = tid & 31;
   int pos = 0, page = -1;
-  if (r0 + lane < P.rows) { page = page_of_row(P, r0 + lane, pos); if ((pos + 1) & (P.R.page - 1)) page = -1; }
+  if (r0 + lane < P.rows) { page = page_of_row(P, r0 + lane, pos); if ((pos & (P.R.page - 1)) != P.R.page - 1) page = -1; }
   unsigned todo = __ballot_sync(0xffffffffu, page >= 0);               // the same in every warp of the block
   while (todo) {
     const int which = __ffs(todo) - 1, pg = __shfl_sync(0xffffffffu, page, which), end = __shfl_sync(0xffffffffu, pos, which), first = end - P.R.page + 1;
