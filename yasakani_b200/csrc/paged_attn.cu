@@ -73,12 +73,6 @@ __device__ __forceinline__ void ldm4t(uint32_t a, uint32_t (&r)[4]) {
 __device__ __forceinline__ void stm2t(uint32_t a, uint32_t x, uint32_t y) {
   asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1,%2};" ::"r"(a), "r"(x), "r"(y) : "memory");
 }
-template <bool BF> __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if (BF) asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-              : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-           : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // Tokens of a row that this kernel attends to by position: [start, vis); a row that has all of the shared prefix leaves that to the prefix kernel.
@@ -284,7 +278,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
           uint32_t a[4];
           ldm4(a0 + (cc >> 3) * (chunk * 128) + (((cc & 7) ^ (r & 7)) << 4), a);
           #pragma unroll
-          for (int n = 0; n < NT; ++n) mma<BF>(c[n][ks & 1], a, qf[n][ks][0], qf[n][ks][1]);
+          for (int n = 0; n < NT; ++n) mma<BF>(c[n][ks & 1], a[0], a[1], a[2], a[3], qf[n][ks][0], qf[n][ks][1]);
         }
       }
       // tokens of the tile that the row sees: lane row g8 and g8 + 8 of this warp's
@@ -347,7 +341,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constan
             ldm4t(sv + ch * (chunk * HD * 2) + (cc >> 3) * (chunk * 128) + r * 128 + (((cc & 7) ^ (r & 7)) << 4), a);
             a[0] &= keep0; a[1] &= keep0; a[2] &= keep1; a[3] &= keep1;
             #pragma unroll
-            for (int n = 0; n < NT; ++n) mma<BF>(o[n][y], a, pf[n][2 * ks], pf[n][2 * ks + 1]);
+            for (int n = 0; n < NT; ++n) mma<BF>(o[n][y], a[0], a[1], a[2], a[3], pf[n][2 * ks], pf[n][2 * ks + 1]);
           }
         }
       }
