@@ -452,9 +452,10 @@ YSKN_KV4_API int yskn_kv4_paged_append(const yskn_paged_cache* c, const yskn_pag
 
 /* The blocks that a row attends to, chosen by a cheap score.  Of the blocks in front of the row's last one (block pos / page, which is always taken) the
  * `take` - 1 with the highest score, ties to the lowest block: score = max over the heads h of the kv-head's group of q_h . kmean[page], summed in fp64 (a
- * score that is not a number counts as the lowest; blocks without a page are no candidates).  ids [rows][kvh][take]: the chosen blocks in rising order, then -1;
+ * score that is not a number counts as the lowest; blocks without a page are no candidates).  Such a sum is exact, and the choice the same in any order of summation, while the products that are
+ * not zero lie within a factor of 2^23 (fp16) or 2^29 (bf16) of one another; otherwise scores closer than 2^-41 of the largest product may be ranked by rounding.  ids [rows][kvh][take]: the chosen blocks in rising order, then -1;
  * for a padding row nothing is written, for a row at a negative position all -1.  A position beyond the table counts as the table's last.  q: rows [nh][hd] of the
- * cache's type at a distance of q_stride elements, 16-byte aligned.  2 <= take <= 1024; nh / kvh <= 16. */
+ * cache's type at a distance of q_stride elements, 16-byte aligned.  2 <= take <= 1024; nh / kvh <= 16; at most 65535 rows. */
 typedef struct yskn_paged_select_args {
   const void* q; int64_t q_stride; int nh, take;
   int* ids; void* workspace; size_t workspace_bytes;
@@ -462,7 +463,7 @@ typedef struct yskn_paged_select_args {
 YSKN_KV4_API int yskn_kv4_paged_select(const yskn_paged_cache* c, const yskn_paged_rows* r, const yskn_paged_select_args* a, void* cuda_stream);
 
 /* Attention of every row over the tokens 0 .. pos of its sequence: o16 [rows][nh][hd] = softmax(qscale * q . k) v, statistics and sums in fp32, weights rounded
- * to the cache's type for the products.  q: rows [nh][hd] (rotated) at a distance of q_stride elements.  nh / kvh <= 16.  A position beyond the table counts as the
+ * to the cache's type for the products.  q: rows [nh][hd] (rotated) at a distance of q_stride elements.  nh / kvh <= 16; at most 65535 rows.  A position beyond the table counts as the
  * table's last; tokens without a page are not seen; a row that sees nothing becomes zeros; a padding row is left as it is.  What pages hold beyond a
  * sequence's tokens is never used, whatever it is.
  *   shared > 0  (a multiple of page): the first `shared` tokens lie on the same pages in the table of every row that has that many (read through the first

@@ -1,13 +1,16 @@
 // Choice of the blocks that a row attends to (sm_100a): a score for every complete page, then the highest ones.
 //
-// Mathematics: score(b) = max over the heads h of a kv-head's group of sum_c q_h[c] mean_b[c].  The choice is the one that fp64 sums make: products of two 16-bit values
-// are exact there, and a sum of HD of them is exact or off by 2^-52 of its largest part, so that the choice depends on no order of a sum.  fp64 sums of everything
+// Mathematics: score(b) = max over the heads h of a kv-head's group of sum_c q_h[c] mean_b[c].  The choice is the one that fp64 sums make.  Products of two 16-bit values are
+// exact there (22 bits at most), and so is a sum of 256 of them, in any order, while those that are not zero lie within a factor of 2^23 (fp16) or 2^29 (bf16, 16 bits) of one another.  Beyond that a sum
+// is off by 2^-42 of the largest product at most (eight sums of a lane, five over lanes), and blocks whose scores differ by less than 2^-41 of it stand in the order that exact_key's sums give them: four to eight channels a
+// lane in turn, then lanes 16, 8, 4, 2 and 1 apart.  Equal mean keys have equal scores always.  fp64 sums of everything
 // were fp64-bound, though (16 rows of 7 heads over 65,536 tokens: 28 us for 15 MB of mean keys).  So:
 //   1. scores on the tensor cores: exact products, fp32 sums, off by at most e = HD 2^-21 * max over blocks and heads of sum_c |q_h[c] mean_b[c]|, which a second
 //      product yields (HD / 16 instructions of 16 products and a sum each, truncated at 2^-23 of the largest: (17/16) HD 2^-23 of that sum; a factor of about four is margin);
 //   2. with t the (take - 1)-th highest of them: what is above t + 2e is among the chosen, what is below t - 2e is not, for at least take - 1 exact scores are
 //      t - e or more, and at most take - 2 are above t + e; what lies between, a block or two, is scored in fp64.
-// Where a score or e is not finite everything is scored in fp64.
+// Where a score or e is not finite everything is scored in fp64, as are scores that are all equal: by one thread block a (row, kv-head), 198 us for 2,048 blocks of eight heads of 128 channels
+// and 1.66 ms for 16,383, in place of 13 and 17.
 //
 // Bound: the mean keys, 2 HD bytes a page and kv-head, read once per row; in practice latency: from one launch to the next a chain of five dependent reads (position, table,
 // means; scores, page) and six block-wide steps.  2,048 blocks of one row: scores 3.7 us, choice 7 us (with fp64 scores of all blocks and a choice by 8-bit digits: 31 and 14 us for
@@ -220,7 +223,7 @@ template <int HD, bool BF> __device__ u64 exact_key(const SelectP& P, const Plac
 }
 
 // The choice, a thread block a (row, kv-head).  PER blocks a thread stay in registers: 8, or 32 where a table has more than 4,096 (16,383 blocks of one row read again for each walk: with
-// scores and attention 44.5 us, kept 30.5).
+// scores and attention 44.5 us, kept 30.5; 32 of 256 channels in bf16 leave 96 bytes of a thread outside its registers).
 template <int HD, bool BF, int PER>
 __global__ void __launch_bounds__(CT, 1) paged_choose_kernel(const SelectP P) {
   __shared__ Shared sh;
