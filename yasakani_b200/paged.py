@@ -85,5 +85,5 @@ def launch_select(q, cache: PagedCache, table, seq, pos, ids, ws, stream=None) -
 
 def launch_attention(q, cache: PagedCache, table, seq, pos, qscale: float, o16, ws, shared: int = 0, blocks=None, stream=None) -> None:
     """Attention of every row over tokens 0 .. pos of its sequence into o16 [rows][nh][hd] (yskn_kv4_paged_attention).  shared: so many first tokens lie on the same
-    pages for every row, and are read once for all.  blocks: int32 [rows][hkv][take], the only blocks that a row sees (launch_select)."""
+    pages for every row, and are read once for all: a common prompt, or what lies in front of a chunk of one sequence whose rows these are.  blocks: int32 [rows][hkv][take], the only blocks that a row sees (launch_select)."""
     host.paged_attention(cache.c, cache.k, table, seq, pos, q, qscale, o16, shared, blocks, ws, stream)
