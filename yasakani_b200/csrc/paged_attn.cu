@@ -535,7 +535,8 @@ int launch_paged_attention(const yskn_paged_cache& c, const yskn_paged_rows& r, 
             w.span, w.ml, w.pacc, w.qml + part, w.qacc + part * c.hd, splits, splits > 0 && first == 0 ? 1 : 0};
     if (int rc = c.hd == 256 ? dispatch<256>(c, P, st) : dispatch<128>(c, P, st)) return rc;
     // Few rows have many parts: eight warps each, a block an SM at most, since blocks of this launch lie beside the attention kernel's from early on and a second wave of them
-    // would start when all is over (five rows of 24 heads over 48 blocks with their choice 31.8 us, 240 blocks of 256 channels' halves, and 25.7 with 30).  More have few parts:
+    // would start when all is over (five rows of 24 heads over 48 blocks with their choice 31.8 us, 240 blocks of 256 channels' halves, and 25.7 with 30).  Between events of a graph, eight warps and one, rows of 28 heads of 128 over 1,000 tokens: 28 items 7.3 us and 8.2, 140 8.7 and 9.7, and beyond the border 168 8.8 and
+    // 9.7, 224 9.2 and 9.7, 280 10.2 and 10.1, 336 13.4 and 11.4; over 8,000 tokens 28 items 10.5 and 18.1, 140 21.8 and 23.0, 280 34.5 and 35.2, 336 41.4 and 40.0.  More have few parts:
     // a warp, which asks for eight at once where there are SMs for all of them (16 rows of 28 heads over 33 blocks 33.6 us, four at once 34.7), and for
     // four where its registers count (200 rows of 28 heads behind 5,216 tokens 62.4 us, eight 63.7)
     const bool bf = c.dtype == YSKN_KV4_BF16;

@@ -456,8 +456,12 @@ int prefix_status_fetch(int* out) {
 }  // namespace paged
 
 // Runs of the prefix for so many pairs of CTAs a kv-head: one wave of them where that goes, else what fills the waves best, a run's start and end counted as a
-// twentieth of a prefix.  It depends on the prefix only in that a run has two tiles at least (one: a short prefix takes the SMs from the rows' own part beside it, 8 rows
-// behind 4,096 tokens 14.9 us, with two 12.3, three 13.2, four 14.0), so that a workspace for many rows and tokens serves fewer.
+// twentieth of a prefix.  It depends on the prefix only in that a run has two tiles at least, so that a workspace for many rows and tokens serves fewer.  Both rules are compromises:
+//   two tiles  (2 to 100 rows, 200 tokens of their own, us with one / two / three tiles at least) gains where one tile a run takes the SMs from the rows' own part beside it, loses a little where it
+//              leaves them idle, and from 8,192 tokens (256 channels) or 16,384 (128) on nothing of it is felt: 28 heads of 128, eight rows: behind 512 tokens 10.1 / 10.8 / 10.8, behind 2,048 16.0 / 11.7 / 12.4, behind
+//              4,096 17.0 / 16.9 / 16.1; 24 heads of 256, 32 rows: behind 512 25.2 / 25.3 / 25.0, behind 2,048 30.0 / 26.8 / 27.6, behind 4,096 31.7 / 31.5 / 29.2
+//   a twentieth (64 heads over eight of 128 channels, us with 1 / 2 / 3 / 4 runs) is about right for long prefixes, too little for short ones: 80 pairs of CTAs (four by the rule) behind 16,384 tokens
+//              275 / 230 / 221 / 225, behind 2,048 87 / 89 / 95 / 108; 128 (one) 311 / 324 / 342 / 335 and 117 / 133 / 149 / 165; 192 (three) 484 / 501 / 492 / 530 and 174 / 199 / 214 / 246
 static int prefix_runs(long long pairs, int kvh) {
   const long long items = pairs * kvh, slots = paged::SMS / 2;
   if (items <= slots) return (int)std::min<long long>(paged::MAX_SPLITS, slots / items);
