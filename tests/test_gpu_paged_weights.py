@@ -75,3 +75,22 @@ def test_scores_that_fp32_holds_in_large_steps(dt, shared, size):
     for scale in (1.0, -1.0):
         o16, _ = attend(k, v, torch.arange(k.shape[0], dtype=torch.int32, device="cuda")[None].contiguous(), ints([0] * 3), ints([n - 1] * 3), q, scale, shared=shared)
         assert (o16 >= 1.0 - 2 * h).all() and (o16 <= 2.0 * (1 + 2 * h)).all(), (float(o16.min()), float(o16.max()))
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("shared", [0, 640])
+@pytest.mark.parametrize("at", [3, 600, 700])
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_a_score_that_is_not_finite_is_not_lost(dt, shared, at, what):
+    """A softmax with a score that is no number, or infinite, has no value: the heads that see such a key say so, rows that end in front of it and the other kv-head do not."""
+    g = torch.Generator(device="cuda").manual_seed(at)
+    n, hkv, nh, hd = 800, 2, 14, 128
+    k = torch.randn((-(-n // 64), hkv, 64, hd), generator=g, device="cuda").to(DT[dt])
+    v = torch.randn(k.shape, generator=g, device="cuda").to(DT[dt])
+    k[at // 64, 1, at % 64, 5] = what
+    q = torch.randn((3, nh, hd), generator=g, device="cuda").to(DT[dt])
+    q[..., 5] = 1.0
+    o16, _ = attend(k, v, torch.arange(k.shape[0], dtype=torch.int32, device="cuda")[None].contiguous(), ints([0] * 3), ints([n - 1, at, at - 1]), q, 0.1, shared=shared)
+    assert torch.isnan(o16[:2, nh // 2:]).all()
+    assert torch.isfinite(o16[:, :nh // 2]).all()
+    assert torch.isfinite(o16[2]).all()
